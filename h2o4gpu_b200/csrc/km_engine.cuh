@@ -223,7 +223,10 @@ struct Engine : EngineBase {
   int assign_all(int flags, bool closes_fit = false);
   // waits for passes with nothing queued behind them and makes them again on whole rows if need be (*again)
   int settle_alone(bool* again = nullptr);
+  template <typename Sink>
+  int distance_blocks(int local, const Sink& sink);
   int transform_shard(int local, T* out_host, size_t ld);
+  int nearest_shard(int local, int n, float scale, bool over_all, int* ids, float* weights, float* best, float* total);
   int inertia(double* out);
   int inertia_launch();
   int inertia_collect(double* out);

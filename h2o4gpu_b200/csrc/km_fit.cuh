@@ -546,14 +546,13 @@ int Engine<T>::inertia_collect(double* out) {
   return KM_OK;
 }
 
-// Squared distances of one shard, column-major with leading dimension ld, to the host.
+// Squared distances of one shard in blocks of rows, each column-major on the device: sink(first row, rows, block, leading
+// dimension) gets them on the shard's stream, behind the kernels that made them, and leaves the block free to be written again
+// by what follows on the stream.
 template <typename T>
-int Engine<T>::transform_shard(int local, T* out_host, size_t ld) {
-  TraceRange trace_range("kmeans.transform");
-  if (local < 0 || local >= (int)shards.size() || !out_host) KM_FAIL(KM_EINVAL, "kmeans_transform_resident: bad argument");
-  if (!have_centroids) KM_FAIL(KM_ESTATE, "no centroids set");
+template <typename Sink>
+int Engine<T>::distance_blocks(int local, const Sink& sink) {
   Shard<T>& s = shards[local];
-  if (ld < s.rows) KM_FAIL(KM_EINVAL, "kmeans_transform_resident: ld smaller than the shard");
   // max|x| (the tensor-core kernel's operand scale) is known after the data check; with several
   // processes that check is a collective and is left to the fit
   if (world_size == (int)shards.size()) KM_TRY(check_data());
@@ -573,8 +572,6 @@ int Engine<T>::transform_shard(int local, T* out_host, size_t ld) {
   cudaEventCreate(&e1);
   float ms_kernels = 0;
   int rc = KM_OK;
-  // below 16 MB the copy is over before the workers have started
-  const bool stage_result = host_pointer_is_pageable(out_host);
   bool wide = false, streamed = false;
   if constexpr (std::is_same<T, float>::value) {
     // tensor-core kernels with a store epilogue (they need max|x| for the operand scales, i.e. a checked
@@ -614,23 +611,10 @@ int Engine<T>::transform_shard(int local, T* out_host, size_t ld) {
     if (!wide && !streamed) rc = launch_tiles(s, s.X + r * (size_t)d, nr, nullptr, MODE_TRANSFORM, buf, batch, false);
     if (rc != KM_OK) break;
     cudaEventRecord(e1, s.stream);
-    cudaError_t ce = cudaSuccess;
-    int staged = KM_ENOMEM;
-    if (stage_result && nr * (size_t)k * sizeof(T) >= ((size_t)16 << 20)) {
-      ce = cudaStreamSynchronize(s.stream);
-      if (ce == cudaSuccess)
-        staged = stage_out(s.dev, reinterpret_cast<const unsigned char*>(buf), batch * sizeof(T),
-                           reinterpret_cast<unsigned char*>(out_host + r), ld * sizeof(T), nr * sizeof(T), (size_t)k);
-      if (ce == cudaSuccess && staged != KM_OK && staged != KM_ENOMEM) { rc = staged; break; }
-    }
-    if (ce == cudaSuccess && staged != KM_OK) {
-      ce = cudaMemcpy2DAsync(out_host + r, ld * sizeof(T), buf, batch * sizeof(T), nr * sizeof(T), k,
-                             cudaMemcpyDeviceToHost, s.stream);
-      if (ce == cudaSuccess) ce = cudaStreamSynchronize(s.stream);
-    }
-    if (ce != cudaSuccess) { set_error(std::string("transform copy: ") + cudaGetErrorString(ce)); rc = KM_ECUDA; }
+    rc = sink(r, nr, buf, batch);
+    if (rc != KM_OK) break;
     float ms = 0;
-    if (cudaEventElapsedTime(&ms, e0, e1) == cudaSuccess) ms_kernels += ms;
+    if (cudaEventSynchronize(e1) == cudaSuccess && cudaEventElapsedTime(&ms, e0, e1) == cudaSuccess) ms_kernels += ms;
   }
   cudaEventDestroy(e0);
   cudaEventDestroy(e1);
@@ -640,6 +624,55 @@ int Engine<T>::transform_shard(int local, T* out_host, size_t ld) {
   }
   km_free(buf);
   return rc;
+}
+
+// Squared distances of one shard, column-major with leading dimension ld, to the host.
+template <typename T>
+int Engine<T>::transform_shard(int local, T* out_host, size_t ld) {
+  TraceRange trace_range("kmeans.transform");
+  if (local < 0 || local >= (int)shards.size() || !out_host) KM_FAIL(KM_EINVAL, "kmeans_transform_resident: bad argument");
+  if (!have_centroids) KM_FAIL(KM_ESTATE, "no centroids set");
+  Shard<T>& s = shards[local];
+  if (ld < s.rows) KM_FAIL(KM_EINVAL, "kmeans_transform_resident: ld smaller than the shard");
+  // below 16 MB the copy is over before the workers have started
+  const bool stage_result = host_pointer_is_pageable(out_host);
+  return distance_blocks(local, [&](size_t r, size_t nr, T* buf, size_t batch) -> int {
+    cudaError_t ce = cudaSuccess;
+    int staged = KM_ENOMEM;
+    if (stage_result && nr * (size_t)k * sizeof(T) >= ((size_t)16 << 20)) {
+      ce = cudaStreamSynchronize(s.stream);
+      if (ce == cudaSuccess)
+        staged = stage_out(s.dev, reinterpret_cast<const unsigned char*>(buf), batch * sizeof(T),
+                           reinterpret_cast<unsigned char*>(out_host + r), ld * sizeof(T), nr * sizeof(T), (size_t)k);
+      if (ce == cudaSuccess && staged != KM_OK && staged != KM_ENOMEM) return staged;
+    }
+    if (ce == cudaSuccess && staged != KM_OK) {
+      ce = cudaMemcpy2DAsync(out_host + r, ld * sizeof(T), buf, batch * sizeof(T), nr * sizeof(T), k,
+                             cudaMemcpyDeviceToHost, s.stream);
+      if (ce == cudaSuccess) ce = cudaStreamSynchronize(s.stream);
+    }
+    if (ce != cudaSuccess) { set_error(std::string("transform copy: ") + cudaGetErrorString(ce)); return KM_ECUDA; }
+    return KM_OK;
+  });
+}
+
+// The n nearest clusters of one shard's rows and their weights, from the same blocks, without the host.
+template <typename T>
+int Engine<T>::nearest_shard(int local, int n, float scale, bool over_all, int* ids, float* weights, float* best, float* total) {
+  TraceRange trace_range("kmeans.nearest");
+  if (!std::is_same<T, float>::value) KM_FAIL(KM_EINVAL, "kmeans_nearest_resident: float32 handles");
+  if (local < 0 || local >= (int)shards.size() || !ids || !weights || !best || !total)
+    KM_FAIL(KM_EINVAL, "kmeans_nearest_resident: bad argument");
+  if (world_size != (int)shards.size()) KM_FAIL(KM_EINVAL, "kmeans_nearest_resident: handles of one process");
+  if (!have_centroids) KM_FAIL(KM_ESTATE, "no centroids set");
+  Shard<T>& s = shards[local];
+  KM_TRY(distance_blocks(local, [&](size_t r, size_t nr, T* buf, size_t batch) -> int {
+    return kmeans_route(KM_DTYPE_F32, buf, 1, (long long)batch, nr, k, n, scale, over_all, ids + r * n, weights + r * n, best + r,
+                        total + r, s.stream);
+  }));
+  DevGuard g(s.dev);
+  KM_CUDA(cudaStreamSynchronize(s.stream));
+  return KM_OK;
 }
 
 }  // namespace km

@@ -1,0 +1,101 @@
+// Shared by the row operators (kmeans_rows.cu): element types, argument checks, launch helpers.
+#pragma once
+
+#include <cuda_bf16.h>
+
+#include <cmath>
+#include <exception>
+
+#include "km_common.cuh"
+
+namespace km {
+namespace rows {
+
+// ---- elements -----------------------------------------------------------------
+// Everything is computed in float32; a value is rounded once, to nearest, when it is stored.
+template <typename T> __device__ __forceinline__ float to_f(T v);
+template <> __device__ __forceinline__ float to_f<float>(float v) { return v; }
+template <> __device__ __forceinline__ float to_f<__half>(__half v) { return __half2float(v); }
+template <> __device__ __forceinline__ float to_f<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <typename T> __device__ __forceinline__ T from_f(float v);
+template <> __device__ __forceinline__ float from_f<float>(float v) { return v; }
+template <> __device__ __forceinline__ __half from_f<__half>(float v) { return __float2half_rn(v); }
+template <> __device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+__device__ __forceinline__ float warp_sum_f(float v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+// Sum over the CTA, the same in every thread; `red` holds 32 floats and may be used again after the next barrier.
+__device__ __forceinline__ float cta_sum(float v, float* red) {
+  v = warp_sum_f(v);
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+  __syncthreads();
+  float s = (threadIdx.x & 31) < (blockDim.x >> 5) ? red[threadIdx.x & 31] : 0.f;
+  s = warp_sum_f(s);
+  __syncthreads();
+  return s;
+}
+
+// ---- host side ----------------------------------------------------------------
+inline int elem_size(int dtype) {
+  switch (dtype) {
+    case KM_DTYPE_F32: return 4;
+    case KM_DTYPE_F16: return 2;
+    case KM_DTYPE_BF16: return 2;
+    default: return 0;
+  }
+}
+inline bool aligned(const void* p, size_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; }
+
+// A row-major block the caller passes: pointer, row stride in elements.  Row starts must fit 63 bits of bytes.
+inline bool block_ok(const void* p, long long stride, size_t rows, size_t cols, int size, bool output) {
+  if (!p || !aligned(p, size) || stride < 0) return false;
+  if (output && rows > 1 && (unsigned long long)stride < cols) return false;   // rows would overlap
+  return rows <= 0x7fffffffULL && cols <= 0x7fffffffULL && (unsigned long long)stride <= (1ULL << 31);
+}
+
+// Multiprocessors of the current device, asked once per device.
+inline int sm_count(int* out) {
+  static std::mutex m;
+  static int count[64] = {};
+  int dev = 0;
+  cudaError_t ce = cudaGetDevice(&dev);
+  if (ce == cudaErrorNoDevice || ce == cudaErrorInsufficientDriver) KM_FAIL(KM_ENODEV, "no CUDA device visible");
+  KM_CUDA(ce);
+  if (dev < 0 || dev >= 64) KM_FAIL(KM_ENODEV, "device index out of range");
+  std::lock_guard<std::mutex> lock(m);
+  if (count[dev] == 0) KM_CUDA(cudaDeviceGetAttribute(&count[dev], cudaDevAttrMultiProcessorCount, dev));
+  *out = count[dev];
+  return KM_OK;
+}
+
+// What a C entry point runs: nothing may leave it but a code.
+template <typename F>
+int guarded(const char* name, F&& f) noexcept {
+  try {
+    return f();
+  } catch (const std::bad_alloc&) {
+    return KM_ENOMEM;
+  } catch (const std::exception& e) {
+    try { set_error(std::string(name) + ": " + e.what()); } catch (...) {}
+    return KM_EINVAL;
+  } catch (...) {
+    return KM_EINVAL;
+  }
+}
+
+#define KM_ROWS_DTYPE(dtype, T, ...)                                     \
+  do {                                                                   \
+    switch (dtype) {                                                     \
+      case KM_DTYPE_F32: { using T = float; __VA_ARGS__; } break;        \
+      case KM_DTYPE_F16: { using T = __half; __VA_ARGS__; } break;       \
+      case KM_DTYPE_BF16: { using T = __nv_bfloat16; __VA_ARGS__; } break; \
+      default: break;                                                    \
+    }                                                                    \
+  } while (0)
+
+}  // namespace rows
+}  // namespace km

@@ -614,6 +614,12 @@ int kmeans_transform_resident(kmeans_handle_t h, int local, void* out, size_t ld
               h->f64->transform_shard(local, static_cast<double*>(out), ld));
 }
 
+int kmeans_nearest_resident(kmeans_handle_t h, int local, int n, float scale, int over_all, int32_t* ids, float* weights,
+                            float* best, float* total) {
+  KM_DISPATCH(h, h->f32->nearest_shard(local, n, scale, over_all != 0, ids, weights, best, total),
+              h->f64->nearest_shard(local, n, scale, over_all != 0, ids, weights, best, total));
+}
+
 int kmeans_get_stats(kmeans_handle_t h, kmeans_stats* out) {
   KM_DISPATCH(h, get_stats(h->f32, out, 0), get_stats(h->f64, out, 0));
 }

@@ -40,6 +40,7 @@ class ResidentKMeans(object):
         self.k = None
         self.cols = None
         self._rows = [0] * len(devices)
+        self._devices = devices
 
     @staticmethod
     def nccl_unique_id():
@@ -144,6 +145,20 @@ class ResidentKMeans(object):
         out = np.empty(rows * self.k, dtype=self.dtype)
         _lk.check(self._lib.kmeans_transform_resident(self._h, local, out.ctypes.data_as(ctypes.c_void_p), rows))
         return out.reshape((rows, self.k), order='F')
+
+    def shard_rows(self, local=0):
+        """Rows of one shard."""
+        return self._rows[local]
+
+    def shard_device(self, local=0):
+        """CUDA device id of one shard."""
+        return self._devices[local]
+
+    def nearest(self, ids_ptr, weights_ptr, best_ptr, total_ptr, n, scale=-1.0, over_all=0, local=0):
+        """The n nearest clusters of one shard's rows and their weights, into device memory (``rows.nearest`` makes the
+        tensors)."""
+        _lk.check(self._lib.kmeans_nearest_resident(self._h, local, n, scale, over_all, ids_ptr, weights_ptr, best_ptr,
+                                                    total_ptr))
 
     def stats(self):
         st = _lk.Stats()

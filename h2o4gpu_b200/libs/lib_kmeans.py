@@ -21,6 +21,7 @@ LIB_PATH = os.environ.get("H2O4GPU_KM_LIB") or os.path.join(os.path.dirname(_HER
 _c = ctypes
 _sz = _c.c_size_t
 _vp = _c.c_void_p
+_ll = _c.c_longlong
 
 
 ENONFINITE = -6      # KM_ENONFINITE
@@ -85,6 +86,21 @@ SIGNATURES = {
     "kmeans_centroid_sums_f32": (_c.c_int, [_c.c_int, _vp, _vp, _sz, _sz, _c.c_int, _vp, _vp]),
     "kmeans_centroid_sums_f64": (_c.c_int, [_c.c_int, _vp, _vp, _sz, _sz, _c.c_int, _vp, _vp]),
     "kmeans_centroid_sums_noalloc_f32": (_c.c_int, [_vp, _vp, _sz, _sz, _c.c_int, _vp, _vp, _vp]),
+    "kmeans_layer_norm": (_c.c_int, [_c.c_int, _vp, _ll, _sz, _sz, _vp, _vp, _c.c_int, _c.c_double, _vp, _ll, _vp, _vp, _vp]),
+    "kmeans_layer_norm_grad_workspace": (_c.c_int, [_sz, _sz, _c.POINTER(_sz)]),
+    "kmeans_layer_norm_grad": (_c.c_int, [_c.c_int, _vp, _ll, _vp, _ll, _vp, _vp, _sz, _sz, _vp, _c.c_int, _vp, _ll, _vp, _vp,
+                                          _vp, _sz, _vp]),
+    "kmeans_route": (_c.c_int, [_c.c_int, _vp, _ll, _ll, _sz, _c.c_int, _c.c_int, _c.c_float, _c.c_int, _vp, _vp, _vp, _vp,
+                                _vp]),
+    "kmeans_route_grad": (_c.c_int, [_c.c_int, _vp, _vp, _ll, _ll, _sz, _c.c_int, _c.c_int, _c.c_float, _c.c_int, _vp, _vp,
+                                     _vp, _vp, _vp, _ll, _ll, _vp]),
+    "kmeans_nearest_resident": (_c.c_int, [_vp, _c.c_int, _c.c_int, _c.c_float, _c.c_int, _vp, _vp, _vp, _vp]),
+    "kmeans_sort_rows_sizes": (_c.c_int, [_sz, _c.c_int, _c.c_int, _c.c_int, _c.POINTER(_sz), _c.POINTER(_sz)]),
+    "kmeans_sort_rows": (_c.c_int, [_vp, _ll, _sz, _c.c_int, _c.c_int, _c.c_int, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "kmeans_dispatch": (_c.c_int, [_c.c_int, _vp, _ll, _sz, _sz, _c.c_int, _vp, _vp, _sz, _vp, _ll, _vp]),
+    "kmeans_combine": (_c.c_int, [_c.c_int, _vp, _ll, _sz, _sz, _vp, _vp, _sz, _c.c_int, _vp, _ll, _vp]),
+    "kmeans_combine_grad": (_c.c_int, [_c.c_int, _vp, _ll, _vp, _ll, _sz, _sz, _vp, _vp, _vp, _sz, _c.c_int, _vp, _ll, _vp,
+                                       _vp]),
     "kmeans_synth_f32": (_c.c_int, [_c.c_int, _vp, _sz, _sz, _sz, _c.c_int, _vp, _c.c_int, _vp, _c.c_float, _c.c_uint64]),
     "kmeans_synth_f64": (_c.c_int, [_c.c_int, _vp, _sz, _sz, _sz, _c.c_int, _vp, _c.c_int, _vp, _c.c_double, _c.c_uint64]),
 }

@@ -161,6 +161,7 @@ int kmeans_upload_host(kmeans_handle_t h, const void* X, size_t rows, size_t col
 #define KM_DTYPE_U32 8
 #define KM_DTYPE_I64 9
 #define KM_DTYPE_U64 10
+#define KM_DTYPE_BF16 11 /* bfloat16: the row operators of section 5 only */
 int kmeans_upload_host_typed(kmeans_handle_t h, const void* X, int src_dtype, size_t rows, size_t cols,
                              char order);
 
@@ -287,6 +288,92 @@ int kmeans_synth_f32(int gpu_id, float* dX, size_t rows, size_t cols, size_t row
 int kmeans_synth_f64(int gpu_id, double* dX, size_t rows, size_t cols, size_t row0, int kind,
                      const double* centers_host, int n_comp, const double* weights_host,
                      double sigma, uint64_t seed);
+
+/* ---- 5. row operators on device memory (no counterpart in the reference) -----------
+ * What a layer of experts does around a k-means model that routes its rows: rows are normed, their
+ * distances to the centroids become the nearest clusters and weights, rows are sorted by cluster, and
+ * the experts' results are joined again.  Forward and backward.
+ *
+ * All pointers but the size outputs are device memory of the current device; `stream` is a cudaStream_t
+ * (NULL = default stream).  The work is enqueued there: nothing waits, allocates or keeps state between
+ * calls, so calls may be captured into graphs and run at once on several streams, as long as each has
+ * outputs and a workspace of its own.  Rows are float32, float16 or bfloat16 (KM_DTYPE_F32 / _F16 / _BF16), the
+ * elements of a row side by side, rows `stride` elements apart (inputs may repeat a row with stride 0; outputs
+ * may not overlap each other or an input, except where it says so).  Sums and statistics are float32; a value is rounded once,
+ * when it is stored.  Results do not depend on the schedule: the same call gives the same bits.
+ * Arguments are checked before anything is enqueued (KM_EINVAL); rows == 0 is valid and writes what has no rows.
+ * Where `rows * n` entries or their places are counted, they are at most 0x7fff0000. */
+
+/* Layer norm: mean and 1 / sqrt(variance + eps) of each row, y = (x - mean) * rstd * weight + bias.
+ * weight / bias (cols values of param_dtype: float32 or the rows' type) may be NULL, as may mean / rstd (rows
+ * float32 values, which the gradient needs).  y may be x. */
+int kmeans_layer_norm(int dtype, const void* x, long long x_stride, size_t rows, size_t cols, const void* weight,
+                      const void* bias, int param_dtype, double eps, void* y, long long y_stride, float* mean,
+                      float* rstd, void* stream);
+/* Its gradient: dx of the rows' type, dweight and dbias (cols float32 sums over the rows; both or neither).
+ * dx may be dy or x.  The workspace (16-byte aligned; not needed without dweight) holds partial sums and is free
+ * again when the call's work is done. */
+int kmeans_layer_norm_grad_workspace(size_t rows, size_t cols, size_t* bytes);
+int kmeans_layer_norm_grad(int dtype, const void* dy, long long dy_stride, const void* x, long long x_stride,
+                           const float* mean, const float* rstd, size_t rows, size_t cols, const void* weight,
+                           int param_dtype, void* dx, long long dx_stride, float* dweight, float* dbias,
+                           void* workspace, size_t workspace_bytes, void* stream);
+
+/* The n best clusters of each row (1 <= n <= min(k, 32)) and their weights.  scores[row * row_stride + cluster *
+ * col_stride]: distances in transform's column-major layout (row_stride 1), or a linear router's row-major
+ * logits (col_stride 1); other strides work too.  scale > 0: larger scores are better; scale < 0: smaller ones
+ * (distances; scale = -1 / temperature).  Ties go to the lowest cluster; NaN and infinitely bad scores are never
+ * taken, infinitely good ones count as the largest float32.
+ *   z = exp(scale * (score - best)), weight = z / total, total = sum of z over the taken clusters, or over all of
+ *   them (over_all != 0)
+ * ids, weights: rows x n, best first; -1 and 0 where fewer than n can be taken.  best, total: rows (0 and 0 for a
+ * row that can take none). */
+int kmeans_route(int dtype, const void* scores, long long row_stride, long long col_stride, size_t rows, int k,
+                 int n, float scale, int over_all, int32_t* ids, float* weights, float* best, float* total,
+                 void* stream);
+/* d(scores) from d(weights) (rows x n float32), for the outputs of kmeans_route.  dscores, of the scores' type,
+ * lies row after row (dcol_stride 1) or cluster after cluster (drow_stride 1); every one of its rows x k values is
+ * written.  scores, best and total are read with over_all only and may be NULL without. */
+int kmeans_route_grad(int dtype, const float* dweights, const void* scores, long long row_stride,
+                      long long col_stride, size_t rows, int k, int n, float scale, int over_all,
+                      const int32_t* ids, const float* weights, const float* best, const float* total,
+                      void* dscores, long long drow_stride, long long dcol_stride, void* stream);
+
+/* kmeans_route on the distances of shard `local` to the handle's centroids (what kmeans_transform_resident would
+ * write), block after block on the device.  Outputs on the shard's device, rows x n and rows.  float32 handles
+ * of one process.  Runs on the handle's stream and waits for it, as every call on a handle; what the caller's streams
+ * still do with the outputs has to be over before. */
+int kmeans_nearest_resident(kmeans_handle_t h, int local, int n, float scale, int over_all, int32_t* ids,
+                            float* weights, float* best, float* total);
+
+/* Places of rows sorted by cluster.  ids: rows x n (row stride ids_stride; labels of kmeans_labels_device with n = 1,
+ * or ids of kmeans_route); an id outside [0, k) sends the entry nowhere, the same id twice in a row is two entries.
+ * k <= 16384.  Groups follow each other in the clusters' order, each from a multiple of `align` on (tiles of
+ * a matrix product), and keep the entries' order.  Of `capacity` = rows * n + min(k, rows * n) * (align - 1) places:
+ *   offsets[k + 1]  where each cluster's group starts; offsets[k] = places in use, padding included
+ *   counts[k]       entries of each cluster
+ *   slot[rows * n]  place of entry row * n + j, or -1
+ *   source[capacity] entry at a place, or -1 for padding and unused places */
+int kmeans_sort_rows_sizes(size_t rows, int n, int k, int align, size_t* capacity, size_t* workspace_bytes);
+int kmeans_sort_rows(const int32_t* ids, long long ids_stride, size_t rows, int n, int k, int align,
+                     int32_t* offsets, int32_t* counts, int32_t* slot, int32_t* source, void* workspace,
+                     size_t workspace_bytes, void* stream);
+/* out[slot[t * n + j]] = x[t]; places whose source is -1 become zero rows.  Rows of `out` behind `capacity` stay as
+ * they are.  (Places outside [0, capacity) are skipped.) */
+int kmeans_dispatch(int dtype, const void* x, long long x_stride, size_t rows, size_t cols, int n,
+                    const int32_t* slot, const int32_t* source, size_t capacity, void* out, long long out_stride,
+                    void* stream);
+/* y[t] = sum over j of weights[t * n + j] * in[slot[t * n + j]]; entries without a place add nothing, whatever
+ * their weight.  weights (rows x n float32) NULL: all ones, which is the gradient of kmeans_dispatch. */
+int kmeans_combine(int dtype, const void* in, long long in_stride, size_t capacity, size_t cols,
+                   const int32_t* slot, const float* weights, size_t rows, int n, void* y, long long y_stride,
+                   void* stream);
+/* Gradient of kmeans_combine: din[slot[t * n + j]] = weights[t * n + j] * dy[t], zero rows where source is -1;
+ * dweights[t * n + j] = <dy[t], in[slot[t * n + j]]>, 0 without a place. */
+int kmeans_combine_grad(int dtype, const void* dy, long long dy_stride, const void* in, long long in_stride,
+                        size_t capacity, size_t cols, const int32_t* slot, const int32_t* source,
+                        const float* weights, size_t rows, int n, void* din, long long din_stride, float* dweights,
+                        void* stream);
 
 #ifdef __cplusplus
 } /* extern "C" */
