@@ -57,6 +57,11 @@ inline bool block_ok(const void* p, long long stride, size_t rows, size_t cols, 
   return rows <= 0x7fffffffULL && cols <= 0x7fffffffULL && (unsigned long long)stride <= (1ULL << 31);
 }
 
+// Whether every row of a block starts on a 16-byte boundary and is whole pieces of 16 bytes long.
+inline bool rows_aligned(const void* p, long long stride, size_t rows, size_t cols, int size) {
+  return aligned(p, 16) && (cols * size) % 16 == 0 && (rows <= 1 || (stride * size) % 16 == 0);
+}
+
 // Multiprocessors of the current device, asked once per device.
 inline int sm_count(int* out) {
   static std::mutex m;

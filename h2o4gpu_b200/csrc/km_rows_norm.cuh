@@ -1,18 +1,263 @@
 // Layer norm of rows and its gradient.
 //   mu = mean x,  r = 1 / sqrt(mean (x - mu)^2 + eps),  xh = (x - mu) r,  y = xh w + b
 //   g = dy w,  dx = r (g - mean g - xh mean(g xh)),  dw = sum over rows of dy xh,  db = sum over rows of dy
+// Both are bound by memory: a row is read once, kept in registers while its sums are formed, and written once.
 #pragma once
 
-#include "km_rows.cuh"
+#include "km_rows_vec.cuh"
 
 namespace km {
 namespace rows {
 
-constexpr int kNormThreads = 256;
+constexpr int kNormThreads = 256;   // of the kernels for wide rows
 
+// Weights or biases of the columns of piece i (2 H of them), `none` without them.  They stay in L1 from row to row.
+template <typename P, int H, bool ALIGNED>
+__device__ __forceinline__ void load_params(const P* w, int i, int d, float none, float2 (&f)[H]) {
+  constexpr int V = 2 * H;
+  const int c = i * V;
+  if (w == nullptr || c >= d) {
+#pragma unroll
+    for (int e = 0; e < H; ++e) f[e] = both(none);
+    return;
+  }
+  if (ALIGNED) {      // of whole pieces
+    constexpr int PV = Piece<P>::V;
+#pragma unroll
+    for (int h = 0; h < V / PV; ++h) {
+      Piece<P> p;
+      p.q = __ldg(reinterpret_cast<const uint4*>(w + c + h * PV));
+      float2 g[PV / 2];
+      unpack(p, g);
+#pragma unroll
+      for (int e = 0; e < PV / 2; ++e) f[h * (PV / 2) + e] = g[e];
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < H; ++e)
+      f[e] = make_float2(c + 2 * e < d ? to_f(w[c + 2 * e]) : none, c + 2 * e + 1 < d ? to_f(w[c + 2 * e + 1]) : none);
+  }
+}
+
+// How a row is spread: `group` threads (whole warps) take it, NV pieces of 16 bytes each; `per_cta` groups share a CTA.
+struct NormShape {
+  int group = 0;   // 0: too wide, the kernel that reads a row from memory again
+  int nv = 1;
+  int per_cta = 1;
+  int threads() const { return group * per_cta; }
+};
+// One warp while a row is up to 4 pieces a lane (no barrier); wider rows two pieces a thread, then four.  (`most`: what the
+// kernel's registers take.)
+inline NormShape norm_shape(int d, int v, int most) {
+  const int pieces = (d + v - 1) / v;
+  NormShape s;
+  const auto warps = [&](int nv) { return (pieces + 32 * nv - 1) / (32 * nv); };
+  int nv = 0;
+  for (int n = 1; n <= most && !nv; n *= 2)
+    if (warps(n) == 1) nv = n;
+  for (int n = std::min(2, most); n <= most && !nv; n *= 2)
+    if (warps(n) <= 32) nv = n;
+  if (!nv) return s;
+  s.nv = nv;
+  s.group = 32 * warps(nv);
+  s.per_cta = std::max(1, 256 / s.group);
+  return s;
+}
+
+// Barrier among the threads of one group.
+__device__ __forceinline__ void group_sync(int group) {
+  asm volatile("bar.sync %0, %1;" ::"r"((int)threadIdx.x / group + 1), "r"(group) : "memory");
+}
+
+// Mean and sum of squared differences from it.  Each warp takes them of its own columns first - its mean, then the differences - and the
+// warps join by  M2 = sum of M2_w + n_w (mean_w - mean)^2:  no cancellation as in E x^2 - (E x)^2, and one barrier instead of two.
+template <typename T, typename P, int NV, bool ALIGNED>
+__global__ void __launch_bounds__(1024)
+norm_rows_kernel(const T* x, long long xs, int rows, int d, float inv_d, const P* w, const P* b, float eps, T* y, long long ys,
+                 float* mean, float* rstd, int group) {
+  constexpr int V = Piece<T>::V, H = V / 2;
+  __shared__ float2 red[32];
+  const int per_cta = blockDim.x / group, which = threadIdx.x / group, in_group = threadIdx.x - which * group, lane = threadIdx.x & 31;
+  const int t = blockIdx.x * per_cta + which;
+  if (t >= rows) return;      // a whole group
+  const T* xr = x + (long long)t * xs;
+  float2 v[NV][H];
+  {
+    Piece<T> raw[NV];
+#pragma unroll
+    for (int p = 0; p < NV; ++p) raw[p] = load_piece<T, ALIGNED>(xr, p * group + in_group, d);
+#pragma unroll
+    for (int p = 0; p < NV; ++p) unpack(raw[p], v[p]);
+  }
+  float2 s2 = both(0.f);
+#pragma unroll
+  for (int p = 0; p < NV; ++p)
+#pragma unroll
+    for (int e = 0; e < H; ++e) s2 = add2(s2, v[p][e]);
+  float s = warp_sum_f(s2.x + s2.y);
+  // the columns that warp `i` of the group has
+  const auto columns = [&](int i) {
+    int n = 0;
+#pragma unroll
+    for (int p = 0; p < NV; ++p) n += max(0, min(32 * V, d - (p * group + i * 32) * V));
+    return n;
+  };
+  float mu = __fdividef(s, (float)max(1, columns(in_group >> 5)));     // any number near the mean would do here
+  float2 q2 = both(0.f);
+#pragma unroll
+  for (int p = 0; p < NV; ++p) {
+    const int c = (p * group + in_group) * V;
+    if (ALIGNED && c >= d) continue;
+#pragma unroll
+    for (int e = 0; e < H; ++e) {
+      float2 o = add2(v[p][e], both(-mu));
+      if (!ALIGNED) {
+        if (c + 2 * e >= d) o.x = 0.f;
+        if (c + 2 * e + 1 >= d) o.y = 0.f;
+      }
+      q2 = fma2(o, o, q2);
+    }
+  }
+  float q = warp_sum_f(q2.x + q2.y);
+  const int warps = group / 32;
+  if (warps > 1) {
+    if (lane == 0) red[threadIdx.x / 32] = make_float2(s, q);
+    group_sync(group);
+    const float2 o = lane < warps ? red[which * warps + lane] : both(0.f);
+    mu = warp_sum_f(o.x) * inv_d;
+    const int n = lane < warps ? columns(lane) : 0;
+    const float near = __fdividef(o.x, (float)max(1, n)), off = near - mu;
+    q = warp_sum_f(fmaf((float)n * off, off, o.y));
+  } else {
+    // M2 about the mean from M2 about a number near it
+    const float m = s * inv_d, off = m - mu;
+    q = fmaf((float)(-d) * off, off, q);
+    mu = m;
+  }
+  const float r = 1.f / sqrtf(q * inv_d + eps);
+  T* yr = y + (long long)t * ys;
+#pragma unroll
+  for (int p = 0; p < NV; ++p) {
+    const int i = p * group + in_group;
+    float2 wf[H], bf[H];
+    load_params<P, H, ALIGNED>(w, i, d, 1.f, wf);
+    load_params<P, H, ALIGNED>(b, i, d, 0.f, bf);
+#pragma unroll
+    for (int e = 0; e < H; ++e) v[p][e] = fma2(mul2(add2(v[p][e], both(-mu)), both(r)), wf[e], bf[e]);
+    store_piece<T, ALIGNED>(yr, i, d, pack<T>(v[p]));
+  }
+  if (in_group == 0) {
+    if (mean) mean[t] = mu;
+    if (rstd) rstd[t] = r;
+  }
+}
+
+// The gradient.  A group walks through the rows with the grid, so that a thread always has the same columns, and adds their dy xh
+// and dy; the CTA joins its groups in their order and leaves its sums in part[CTA] (dw then db, d each), which
+// norm_grad_sum_kernel adds up in the CTAs' order.
+template <typename T, typename P, int NV, bool ALIGNED>
+__global__ void __launch_bounds__(1024)
+norm_grad_rows_kernel(const T* dy, long long dys, const T* x, long long xs, const float* mean, const float* rstd, int rows, int d,
+                      float inv_d, const P* w, T* dx, long long dxs, float* part, int group) {
+  constexpr int V = Piece<T>::V, H = V / 2;
+  __shared__ float2 red[2][32];      // used in turn: one half may still be read by slower warps
+  const int per_cta = blockDim.x / group, which = threadIdx.x / group, in_group = threadIdx.x - which * group, warps = group / 32;
+  const int lane = threadIdx.x & 31;
+  float2 aw[NV][H], ab[NV][H];
+#pragma unroll
+  for (int p = 0; p < NV; ++p)
+#pragma unroll
+    for (int e = 0; e < H; ++e) aw[p][e] = ab[p][e] = both(0.f);
+  const int step = gridDim.x * per_cta;
+  int t = blockIdx.x * per_cta + which, turn = 0;
+  Piece<T> nx[NV], ng[NV];
+  float nmu = 0.f, nr = 0.f;
+  if (t < rows) {
+#pragma unroll
+    for (int p = 0; p < NV; ++p) {
+      nx[p] = load_piece<T, ALIGNED>(x + (long long)t * xs, p * group + in_group, d);
+      ng[p] = load_piece<T, ALIGNED>(dy + (long long)t * dys, p * group + in_group, d);
+    }
+    nmu = mean[t];
+    nr = rstd[t];
+  }
+  for (; t < rows; t += step, turn ^= 1) {
+    const float mu = nmu, r = nr;
+    float2 xh[NV][H], g[NV][H];
+#pragma unroll
+    for (int p = 0; p < NV; ++p) {
+      unpack(nx[p], xh[p]);
+      unpack(ng[p], g[p]);
+    }
+    if (t + step < rows) {     // the next row is on its way while this one's sums are formed
+#pragma unroll
+      for (int p = 0; p < NV; ++p) {
+        nx[p] = load_piece<T, ALIGNED>(x + (long long)(t + step) * xs, p * group + in_group, d);
+        ng[p] = load_piece<T, ALIGNED>(dy + (long long)(t + step) * dys, p * group + in_group, d);
+      }
+      nmu = mean[t + step];
+      nr = rstd[t + step];
+    }
+    float2 a2 = both(0.f), b2 = both(0.f);
+#pragma unroll
+    for (int p = 0; p < NV; ++p) {
+      float2 wf[H];
+      load_params<P, H, ALIGNED>(w, p * group + in_group, d, 1.f, wf);
+#pragma unroll
+      for (int e = 0; e < H; ++e) {
+        xh[p][e] = mul2(add2(xh[p][e], both(-mu)), both(r));     // behind the row's end g is zero
+        aw[p][e] = fma2(g[p][e], xh[p][e], aw[p][e]);
+        ab[p][e] = add2(ab[p][e], g[p][e]);
+        g[p][e] = mul2(g[p][e], wf[e]);
+        a2 = add2(a2, g[p][e]);
+        b2 = fma2(g[p][e], xh[p][e], b2);
+      }
+    }
+    float s1 = warp_sum_f(a2.x + a2.y), s2 = warp_sum_f(b2.x + b2.y);
+    if (warps > 1) {
+      if (lane == 0) red[turn][threadIdx.x / 32] = make_float2(s1, s2);
+      group_sync(group);
+      const float2 o = lane < warps ? red[turn][which * warps + lane] : both(0.f);
+      s1 = warp_sum_f(o.x);
+      s2 = warp_sum_f(o.y);
+    }
+    const float2 m1 = both(-s1 * inv_d), m2 = both(-s2 * inv_d);
+    T* dr = dx + (long long)t * dxs;
+#pragma unroll
+    for (int p = 0; p < NV; ++p) {
+#pragma unroll
+      for (int e = 0; e < H; ++e) g[p][e] = mul2(both(r), fma2(xh[p][e], m2, add2(g[p][e], m1)));
+      store_piece<T, ALIGNED>(dr, p * group + in_group, d, pack<T>(g[p]));
+    }
+  }
+  if (!part) return;
+  extern __shared__ float joined[];     // dw then db of the CTA, d each
+  float* pw = part + (size_t)blockIdx.x * 2 * d;
+  float* cols = per_cta > 1 ? joined : pw;
+  for (int grp = 0; grp < per_cta; ++grp) {
+    __syncthreads();
+    if (which == grp)
+#pragma unroll
+      for (int p = 0; p < NV; ++p)
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          const int c = (p * group + in_group) * V + e;
+          if (c < d) {
+            const float sw = e & 1 ? aw[p][e / 2].y : aw[p][e / 2].x, sb = e & 1 ? ab[p][e / 2].y : ab[p][e / 2].x;
+            cols[c] = grp ? cols[c] + sw : sw;
+            cols[d + c] = grp ? cols[d + c] + sb : sb;
+          }
+        }
+  }
+  __syncthreads();
+  if (per_cta > 1)
+    for (int c = threadIdx.x; c < 2 * d; c += blockDim.x) pw[c] = cols[c];
+}
+
+// Rows wider than the registers take: one CTA per row, the row read again (from L2) for each of its sums.
 template <typename T, typename P>
 __global__ void __launch_bounds__(kNormThreads)
-norm_kernel(const T* x, long long xs, int d, const P* w, const P* b, float eps, T* y, long long ys, float* mean, float* rstd) {
+norm_wide_kernel(const T* x, long long xs, int d, const P* w, const P* b, float eps, T* y, long long ys, float* mean, float* rstd) {
   __shared__ float red[32];
   const T* xr = x + (long long)blockIdx.x * xs;
   T* yr = y + (long long)blockIdx.x * ys;
@@ -37,16 +282,14 @@ norm_kernel(const T* x, long long xs, int d, const P* w, const P* b, float eps, 
   }
 }
 
-// CTA p of `parts` takes rows p, p + parts, ... and leaves its column sums in part[p] (dw then db, d each).
 template <typename T, typename P>
 __global__ void __launch_bounds__(kNormThreads)
-norm_grad_kernel(const T* dy, long long dys, const T* x, long long xs, const float* mean, const float* rstd, int rows, int d,
-                 const P* w, T* dx, long long dxs, float* part) {
+norm_grad_wide_kernel(const T* dy, long long dys, const T* x, long long xs, const float* mean, const float* rstd, int rows, int d,
+                      const P* w, T* dx, long long dxs, float* part) {
   __shared__ float red[32];
   float* pw = part ? part + (size_t)blockIdx.x * 2 * d : nullptr;
   if (pw)
-    for (int c = threadIdx.x; c < 2 * d; c += kNormThreads) pw[c] = 0.f;
-  __syncthreads();
+    for (int c = threadIdx.x; c < d; c += kNormThreads) pw[c] = pw[d + c] = 0.f;
   for (int t = blockIdx.x; t < rows; t += gridDim.x) {
     const T* xr = x + (long long)t * xs;
     const T* gr = dy + (long long)t * dys;
@@ -73,17 +316,55 @@ norm_grad_kernel(const T* dy, long long dys, const T* x, long long xs, const flo
   }
 }
 
-// dw, db = the parts' sums, in the parts' order.
-__global__ void norm_grad_sum_kernel(const float* part, int parts, int d, float* dw, float* db) {
-  const int c = blockIdx.x * blockDim.x + threadIdx.x;
-  if (c >= 2 * d) return;
+// dw, db = the parts' sums: a warp-wide strip of columns per CTA, 32 runs of consecutive parts, joined in their order.
+__global__ void __launch_bounds__(1024)
+norm_grad_sum_kernel(const float* part, int parts, int d, float* dw, float* db) {
+  __shared__ float run[32][33];
+  const int lane = threadIdx.x, c = blockIdx.x * 32 + lane, per = (parts + 31) / 32;
   float s = 0.f;
-  for (int p = 0; p < parts; ++p) s += part[(size_t)p * 2 * d + c];
-  if (c < d) dw[c] = s;
-  else db[c - d] = s;
+  if (c < 2 * d)
+    for (int p = threadIdx.y * per; p < min(parts, (int)(threadIdx.y + 1) * per); ++p) s += part[(size_t)p * 2 * d + c];
+  run[threadIdx.y][lane] = s;
+  __syncthreads();
+  if (threadIdx.y == 0 && c < 2 * d) {
+    s = 0.f;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) s += run[i][lane];
+    if (c < d) dw[c] = s;
+    else db[c - d] = s;
+  }
 }
 
-inline int norm_grad_parts(size_t rows, int sms) { return (int)std::min<size_t>(rows, (size_t)sms * 2); }
+// CTAs of the gradient's walk, each of which leaves a partial sum: as many as run at once with 64 registers a thread.
+constexpr int kNormGradMost = 2;     // pieces a thread has of float32 rows; 16-bit rows have one
+inline NormShape norm_grad_shape(int d, int size) { return norm_shape(d, 16 / size, size == 4 ? kNormGradMost : 1); }
+inline int norm_grad_grid(size_t rows, const NormShape& s, int sms) {
+  if (!s.group) return (int)std::min<size_t>(rows, (size_t)sms * 4);
+  return (int)std::min<size_t>((rows + s.per_cta - 1) / s.per_cta, (size_t)sms * (1024 / s.threads()));
+}
+
+template <typename T, typename P, bool ALIGNED>
+int norm_launch(const NormShape& s, const T* x, long long xs, int rows, int d, const P* w, const P* b, float eps, T* y,
+                long long ys, float* mean, float* rstd, cudaStream_t stream) {
+  auto fn = s.nv == 1 ? norm_rows_kernel<T, P, 1, ALIGNED> : s.nv == 2 ? norm_rows_kernel<T, P, 2, ALIGNED>
+                                                                       : norm_rows_kernel<T, P, 4, ALIGNED>;
+  fn<<<(rows + s.per_cta - 1) / s.per_cta, s.threads(), 0, stream>>>(x, xs, rows, d, 1.f / (float)d, w, b, eps, y, ys, mean, rstd, s.group);
+  KM_CUDA(cudaGetLastError());
+  return KM_OK;
+}
+
+template <typename T, typename P, bool ALIGNED>
+int norm_grad_launch(const NormShape& s, int grid, const T* dy, long long dys, const T* x, long long xs, const float* mean,
+                     const float* rstd, int rows, int d, const P* w, T* dx, long long dxs, float* part, cudaStream_t stream) {
+  auto fn = norm_grad_rows_kernel<T, P, 1, ALIGNED>;
+  if constexpr (sizeof(T) == 4)
+    if (s.nv == 2) fn = norm_grad_rows_kernel<T, P, 2, ALIGNED>;
+  // several groups a CTA: at most 1024 columns, 8 KB
+  const size_t smem = part && s.per_cta > 1 ? (size_t)2 * d * sizeof(float) : 0;
+  fn<<<grid, s.threads(), smem, stream>>>(dy, dys, x, xs, mean, rstd, rows, d, 1.f / (float)d, w, dx, dxs, part, s.group);
+  KM_CUDA(cudaGetLastError());
+  return KM_OK;
+}
 
 }  // namespace rows
 }  // namespace km

@@ -1,0 +1,168 @@
+// Rows in 16-byte pieces, whatever their alignment.
+// Piece i of a row is its elements [i V, i V + V).  Where rows start on 16-byte boundaries a piece is one load or store.  Elsewhere a
+// piece lies across two aligned words of 16 bytes: a load takes both and shifts (the second is the next lane's first, so it comes from
+// L1), a store passes what does not fit its own word to the next lane.  Words that stick out of the row are taken apart element by
+// element: nothing outside the row is touched.
+#pragma once
+
+#include "km_rows.cuh"
+
+namespace km {
+namespace rows {
+
+template <typename T> struct Piece {
+  static constexpr int V = 16 / (int)sizeof(T);
+  union {
+    uint4 q;
+    unsigned int w[4];
+    T e[V];
+  };
+  __device__ __forceinline__ Piece() {}
+};
+
+// Two float32 operations in one instruction.
+__device__ __forceinline__ unsigned long long as_u64(float2 a) {
+  unsigned long long r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a.x), "f"(a.y));
+  return r;
+}
+__device__ __forceinline__ float2 as_f2(unsigned long long a) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(a));
+  return r;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  unsigned long long r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(as_u64(a)), "l"(as_u64(b)));
+  return as_f2(r);
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  unsigned long long r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(as_u64(a)), "l"(as_u64(b)));
+  return as_f2(r);
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  unsigned long long r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(as_u64(a)), "l"(as_u64(b)), "l"(as_u64(c)));
+  return as_f2(r);
+}
+__device__ __forceinline__ float2 both(float a) { return make_float2(a, a); }
+
+// A piece as pairs of float32 and back (each value rounded once, to nearest).
+template <typename T> __device__ __forceinline__ float2 word_pair(unsigned int w);
+template <> __device__ __forceinline__ float2 word_pair<__nv_bfloat16>(unsigned int w) {
+  return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+template <> __device__ __forceinline__ float2 word_pair<__half>(unsigned int w) {
+  __half2 h;
+  memcpy(&h, &w, 4);
+  return __half22float2(h);
+}
+template <typename T> __device__ __forceinline__ unsigned int pair_word(float2 f);
+template <> __device__ __forceinline__ unsigned int pair_word<__nv_bfloat16>(float2 f) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(f.x, f.y);
+  unsigned int w;
+  memcpy(&w, &h, 4);
+  return w;
+}
+template <> __device__ __forceinline__ unsigned int pair_word<__half>(float2 f) {
+  const __half2 h = __floats2half2_rn(f.x, f.y);
+  unsigned int w;
+  memcpy(&w, &h, 4);
+  return w;
+}
+template <typename T>
+__device__ __forceinline__ void unpack(const Piece<T>& p, float2 (&f)[Piece<T>::V / 2]) {
+  if constexpr (sizeof(T) == 4) {
+    f[0] = make_float2(__uint_as_float(p.w[0]), __uint_as_float(p.w[1]));
+    f[1] = make_float2(__uint_as_float(p.w[2]), __uint_as_float(p.w[3]));
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f[i] = word_pair<T>(p.w[i]);
+  }
+}
+template <typename T>
+__device__ __forceinline__ Piece<T> pack(const float2 (&f)[Piece<T>::V / 2]) {
+  Piece<T> p;
+  if constexpr (sizeof(T) == 4) {
+    p.q = make_uint4(__float_as_uint(f[0].x), __float_as_uint(f[0].y), __float_as_uint(f[1].x), __float_as_uint(f[1].y));
+  } else {
+    p.q = make_uint4(pair_word<T>(f[0]), pair_word<T>(f[1]), pair_word<T>(f[2]), pair_word<T>(f[3]));
+  }
+  return p;
+}
+
+// Bytes [shift, shift + 16) of the 32 bytes a, b.
+__device__ __forceinline__ uint4 shift_words(uint4 a, uint4 b, unsigned int shift) {
+  unsigned int w0 = a.x, w1 = a.y, w2 = a.z, w3 = a.w, w4 = b.x, w5 = b.y, w6 = b.z, w7 = b.w;
+  if (shift & 8) { w0 = w2; w1 = w3; w2 = w4; w3 = w5; w4 = w6; w5 = w7; }
+  if (shift & 4) { w0 = w1; w1 = w2; w2 = w3; w3 = w4; w4 = w5; }
+  const unsigned int bits = (shift & 3) * 8;
+  return make_uint4(__funnelshift_r(w0, w1, bits), __funnelshift_r(w1, w2, bits), __funnelshift_r(w2, w3, bits),
+                    __funnelshift_r(w3, w4, bits));
+}
+
+// Piece i of the row at `row` with d elements; zeros behind the row's end.  ALIGNED: the row starts on a 16-byte boundary and is
+// whole pieces long.
+template <typename T, bool ALIGNED>
+__device__ __forceinline__ Piece<T> load_piece(const T* row, int i, int d) {
+  constexpr int V = Piece<T>::V;
+  Piece<T> p;
+  const int c = i * V;
+  if (ALIGNED) {
+    p.q = c < d ? *reinterpret_cast<const uint4*>(row + c) : make_uint4(0u, 0u, 0u, 0u);
+    return p;
+  } else {
+    const unsigned int off = (unsigned int)(reinterpret_cast<uintptr_t>(row) & 15);
+    // first element of the two words, counted from the row's start, and one behind their last
+    const int first = c - (int)(off / sizeof(T)), behind = first + (off ? 2 : 1) * V;
+    if (first >= 0 && behind <= d) {
+      const uint4* word = reinterpret_cast<const uint4*>(row + first);
+      const uint4 a = word[0];
+      p.q = off ? shift_words(a, word[1], off) : a;
+      return p;
+    }
+  }
+  p.q = make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+  for (int e = 0; e < V; ++e)
+    if (c + e < d) p.e[e] = row[c + e];
+  return p;
+}
+
+// Stores piece i of the row.  Not ALIGNED: all 32 lanes call it with consecutive pieces (lane 0 the first); pieces behind
+// the row's end store nothing.
+template <typename T, bool ALIGNED>
+__device__ __forceinline__ void store_piece(T* row, int i, int d, const Piece<T>& p) {
+  constexpr int V = Piece<T>::V;
+  const int c = i * V;
+  if (ALIGNED) {
+    if (c < d) *reinterpret_cast<uint4*>(row + c) = p.q;
+  } else {
+    const unsigned int off = (unsigned int)(reinterpret_cast<uintptr_t>(row) & 15);   // the same in every lane
+    const int lane = threadIdx.x & 31, m = (int)(off / sizeof(T));
+    // this lane's word: the last m elements of the lane before, then its own first V - m
+    Piece<T> before;
+    before.w[0] = __shfl_up_sync(0xffffffffu, p.w[0], 1);
+    before.w[1] = __shfl_up_sync(0xffffffffu, p.w[1], 1);
+    before.w[2] = __shfl_up_sync(0xffffffffu, p.w[2], 1);
+    before.w[3] = __shfl_up_sync(0xffffffffu, p.w[3], 1);
+    if ((lane > 0 || m == 0) && c + V - m <= d) {
+      *reinterpret_cast<uint4*>(row + c - m) = m ? shift_words(before.q, p.q, 16 - off) : p.q;
+      if (lane < 31 && c + V < d) return;      // the next lane stores the rest
+#pragma unroll
+      for (int e = 0; e < V; ++e)
+        if (e >= V - m && c + e < d) row[c + e] = p.e[e];
+      return;
+    }
+    // the first lane, or a word that sticks out behind the row: the part of the lane before, then the own
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      if (lane > 0 && e >= V - m && c - V + e < d) row[c - V + e] = before.e[e];
+      if (c + e < d && (e < V - m || lane == 31 || c + V >= d)) row[c + e] = p.e[e];
+    }
+  }
+}
+
+}  // namespace rows
+}  // namespace km

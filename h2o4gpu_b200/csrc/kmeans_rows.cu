@@ -41,11 +41,29 @@ int layer_norm(int dtype, const void* x, long long xs, size_t rows, size_t cols,
       !aligned(mean, 4) || !aligned(rstd, 4))
     KM_FAIL(KM_EINVAL, "kmeans_layer_norm: bad argument");
   const int d = (int)cols;
+  const NormShape shape = norm_shape(d, 16 / size, 4);
+  const bool al = rows_aligned(x, xs, rows, cols, size) && rows_aligned(y, ys, rows, cols, size) && aligned(weight, 16) &&
+                  aligned(bias, 16);
+  int rc = KM_OK;
   KM_ROWS_DTYPE(dtype, T, KM_ROWS_PARAM(param_dtype, T, P,
-      norm_kernel<T, P><<<(unsigned)rows, kNormThreads, 0, stream>>>(static_cast<const T*>(x), xs, d, static_cast<const P*>(weight),
-          static_cast<const P*>(bias), (float)eps, static_cast<T*>(y), ys, mean, rstd)));
-  KM_CUDA(cudaGetLastError());
-  return KM_OK;
+      const T* xp = static_cast<const T*>(x);
+      const P* wp = static_cast<const P*>(weight);
+      const P* bp = static_cast<const P*>(bias);
+      T* yp = static_cast<T*>(y);
+      if (!shape.group) {
+        norm_wide_kernel<T, P><<<(unsigned)rows, kNormThreads, 0, stream>>>(xp, xs, d, wp, bp, (float)eps, yp, ys, mean, rstd);
+        KM_CUDA(cudaGetLastError());
+      } else if (al) {
+        rc = norm_launch<T, P, true>(shape, xp, xs, (int)rows, d, wp, bp, (float)eps, yp, ys, mean, rstd, stream);
+      } else {
+        rc = norm_launch<T, P, false>(shape, xp, xs, (int)rows, d, wp, bp, (float)eps, yp, ys, mean, rstd, stream);
+      }));
+  return rc;
+}
+
+// Partial sums of the gradient's walk over rows of `size`-byte elements.
+int norm_grad_parts(size_t rows, size_t cols, int size, int sms) {
+  return norm_grad_grid(rows, norm_grad_shape((int)cols, size), sms);
 }
 
 int layer_norm_grad_workspace(size_t rows, size_t cols, size_t* bytes) {
@@ -54,7 +72,8 @@ int layer_norm_grad_workspace(size_t rows, size_t cols, size_t* bytes) {
   if (rows == 0) return KM_OK;
   int sms = 0;
   KM_TRY(sm_count(&sms));
-  *bytes = (size_t)norm_grad_parts(rows, sms) * 2 * cols * sizeof(float);
+  const int parts = std::max(norm_grad_parts(rows, cols, 2, sms), norm_grad_parts(rows, cols, 4, sms));
+  *bytes = (size_t)parts * 2 * cols * sizeof(float);
   return KM_OK;
 }
 
@@ -79,16 +98,30 @@ int layer_norm_grad(int dtype, const void* dy, long long dys, const void* x, lon
     KM_FAIL(KM_EINVAL, "kmeans_layer_norm_grad: bad argument");
   int sms = 0;
   KM_TRY(sm_count(&sms));
-  const int parts = norm_grad_parts(rows, sms), d = (int)cols;
+  const int parts = norm_grad_parts(rows, cols, size, sms), d = (int)cols;
   if (dweight && (!workspace || !aligned(workspace, 16) || workspace_bytes < (size_t)parts * 2 * cols * sizeof(float)))
     KM_FAIL(KM_EINVAL, "kmeans_layer_norm_grad: workspace missing or too small");
   float* part = dweight ? static_cast<float*>(workspace) : nullptr;
+  const NormShape shape = norm_grad_shape(d, size);
+  const bool al = rows_aligned(x, xs, rows, cols, size) && rows_aligned(dy, dys, rows, cols, size) &&
+                  rows_aligned(dx, dxs, rows, cols, size) && aligned(weight, 16);
+  int rc = KM_OK;
   KM_ROWS_DTYPE(dtype, T, KM_ROWS_PARAM(param_dtype, T, P,
-      norm_grad_kernel<T, P><<<parts, kNormThreads, 0, stream>>>(static_cast<const T*>(dy), dys, static_cast<const T*>(x), xs, mean,
-          rstd, (int)rows, d, static_cast<const P*>(weight), static_cast<T*>(dx), dxs, part)));
-  KM_CUDA(cudaGetLastError());
+      const T* gp = static_cast<const T*>(dy);
+      const T* xp = static_cast<const T*>(x);
+      const P* wp = static_cast<const P*>(weight);
+      T* dp = static_cast<T*>(dx);
+      if (!shape.group) {
+        norm_grad_wide_kernel<T, P><<<parts, kNormThreads, 0, stream>>>(gp, dys, xp, xs, mean, rstd, (int)rows, d, wp, dp, dxs, part);
+        KM_CUDA(cudaGetLastError());
+      } else if (al) {
+        rc = norm_grad_launch<T, P, true>(shape, parts, gp, dys, xp, xs, mean, rstd, (int)rows, d, wp, dp, dxs, part, stream);
+      } else {
+        rc = norm_grad_launch<T, P, false>(shape, parts, gp, dys, xp, xs, mean, rstd, (int)rows, d, wp, dp, dxs, part, stream);
+      }));
+  KM_TRY(rc);
   if (part) {
-    norm_grad_sum_kernel<<<(unsigned)((2 * cols + 255) / 256), 256, 0, stream>>>(part, parts, d, dweight, dbias);
+    norm_grad_sum_kernel<<<(unsigned)((2 * cols + 31) / 32), dim3(32, 32), 0, stream>>>(part, parts, d, dweight, dbias);
     KM_CUDA(cudaGetLastError());
   }
   return KM_OK;
