@@ -28,6 +28,13 @@ __device__ __forceinline__ float warp_sum_f(float v) {
   return v;
 }
 
+// Sum over each half of the warp, the same in all its lanes.
+__device__ __forceinline__ float half_warp_sum(float v) {
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
 // Sum over the CTA, the same in every thread; `red` holds 32 floats and may be used again after the next barrier.
 __device__ __forceinline__ float cta_sum(float v, float* red) {
   v = warp_sum_f(v);

@@ -39,116 +39,118 @@ __device__ __forceinline__ void load_params(const P* w, int i, int d, float none
   }
 }
 
-// How a row is spread: `group` threads (whole warps) take it, NV pieces of 16 bytes each; `per_cta` groups share a CTA.
+// How a row is spread: `group` threads (whole warps) take it, NV pieces of 16 bytes each; `per_cta` groups share a CTA.  A group walks
+// through the rows with the grid, so that a thread always has the same columns.
 struct NormShape {
   int group = 0;   // 0: too wide, the kernel that reads a row from memory again
   int nv = 1;
   int per_cta = 1;
   int threads() const { return group * per_cta; }
 };
-// One warp while a row is up to 4 pieces a lane (no barrier); wider rows two pieces a thread, then four.  (`most`: what the
-// kernel's registers take.)
-inline NormShape norm_shape(int d, int v, int most) {
+// One warp while it can take the row (no barrier), else `most` pieces a thread.
+inline NormShape norm_shape(int d, int v, int most, int max_threads) {
   const int pieces = (d + v - 1) / v;
   NormShape s;
   const auto warps = [&](int nv) { return (pieces + 32 * nv - 1) / (32 * nv); };
-  int nv = 0;
-  for (int n = 1; n <= most && !nv; n *= 2)
-    if (warps(n) == 1) nv = n;
-  for (int n = std::min(2, most); n <= most && !nv; n *= 2)
-    if (warps(n) <= 32) nv = n;
-  if (!nv) return s;
-  s.nv = nv;
-  s.group = 32 * warps(nv);
+  s.nv = pieces <= 32 ? 1 : most;
+  if (32 * warps(s.nv) > max_threads) return s;
+  s.group = 32 * warps(s.nv);
   s.per_cta = std::max(1, 256 / s.group);
   return s;
 }
 
-// Barrier among the threads of one group.
-__device__ __forceinline__ void group_sync(int group) {
-  asm volatile("bar.sync %0, %1;" ::"r"((int)threadIdx.x / group + 1), "r"(group) : "memory");
+// Barrier among the threads of one group: a CTA is group x per_cta threads.
+__device__ __forceinline__ void group_sync() {
+  asm volatile("bar.sync %0, %1;" ::"r"((int)threadIdx.y + 1), "r"((int)blockDim.x) : "memory");
 }
 
 // Mean and sum of squared differences from it.  Each warp takes them of its own columns first - its mean, then the differences - and the
 // warps join by  M2 = sum of M2_w + n_w (mean_w - mean)^2:  no cancellation as in E x^2 - (E x)^2, and one barrier instead of two.
+// A row costs some 8 operations a value on pipes that a memory-bound kernel fills to two thirds, so weights and biases stay in
+// registers (as float32 pairs: unpacking them again for every row was a tenth of the instructions), and the columns' counts are
+// taken before the walk.
+constexpr int kNormMaxThreads = 512;       // a row's group
+constexpr int kNormRegs = 80;              // so that 24 warps fit a processor
+constexpr int kNormThreadsPerSm = 768;
 template <typename T, typename P, int NV, bool ALIGNED>
-__global__ void __launch_bounds__(1024)
+__global__ void __maxnreg__(kNormRegs)
 norm_rows_kernel(const T* x, long long xs, int rows, int d, float inv_d, const P* w, const P* b, float eps, T* y, long long ys,
-                 float* mean, float* rstd, int group) {
+                 float* mean, float* rstd) {
   constexpr int V = Piece<T>::V, H = V / 2;
-  __shared__ float2 red[32];
-  const int per_cta = blockDim.x / group, which = threadIdx.x / group, in_group = threadIdx.x - which * group, lane = threadIdx.x & 31;
-  const int t = blockIdx.x * per_cta + which;
-  if (t >= rows) return;      // a whole group
-  const T* xr = x + (long long)t * xs;
-  float2 v[NV][H];
-  {
-    Piece<T> raw[NV];
-#pragma unroll
-    for (int p = 0; p < NV; ++p) raw[p] = load_piece<T, ALIGNED>(xr, p * group + in_group, d);
-#pragma unroll
-    for (int p = 0; p < NV; ++p) unpack(raw[p], v[p]);
-  }
-  float2 s2 = both(0.f);
-#pragma unroll
-  for (int p = 0; p < NV; ++p)
-#pragma unroll
-    for (int e = 0; e < H; ++e) s2 = add2(s2, v[p][e]);
-  float s = warp_sum_f(s2.x + s2.y);
+  __shared__ float2 red[2][32];      // used in turn: one half may still be read by slower warps
+  const int group = blockDim.x, in_group = threadIdx.x, lane = threadIdx.x & 31, warps = group / 32;
   // the columns that warp `i` of the group has
   const auto columns = [&](int i) {
     int n = 0;
 #pragma unroll
     for (int p = 0; p < NV; ++p) n += max(0, min(32 * V, d - (p * group + i * 32) * V));
-    return n;
+    return (float)n;
   };
-  float mu = __fdividef(s, (float)max(1, columns(in_group >> 5)));     // any number near the mean would do here
-  float2 q2 = both(0.f);
+  const float n_own = columns(in_group / 32), n_lane = (lane & 15) < warps ? columns(lane & 15) : 0.f;
+  const float inv_own = n_own > 0.f ? 1.f / n_own : 0.f, inv_lane = n_lane > 0.f ? 1.f / n_lane : 0.f;
+  float2 wf[NV][H], bf[NV][H];
 #pragma unroll
   for (int p = 0; p < NV; ++p) {
-    const int c = (p * group + in_group) * V;
-    if (ALIGNED && c >= d) continue;
+    load_params<P, H, ALIGNED>(w, p * group + in_group, d, 1.f, wf[p]);
+    load_params<P, H, ALIGNED>(b, p * group + in_group, d, 0.f, bf[p]);
+  }
+  const int step = gridDim.x * blockDim.y;
+  int t = blockIdx.x * blockDim.y + threadIdx.y, turn = 0;
+  Piece<T> next[NV];
+  if (t < rows)
 #pragma unroll
-    for (int e = 0; e < H; ++e) {
-      float2 o = add2(v[p][e], both(-mu));
-      if (!ALIGNED) {
-        if (c + 2 * e >= d) o.x = 0.f;
-        if (c + 2 * e + 1 >= d) o.y = 0.f;
+    for (int p = 0; p < NV; ++p) next[p] = load_piece<T, ALIGNED>(x + (long long)t * xs, p * group + in_group, d);
+  for (; t < rows; t += step, turn ^= 1) {
+    float2 v[NV][H];
+#pragma unroll
+    for (int p = 0; p < NV; ++p) unpack(next[p], v[p]);
+    if (t + step < rows)      // the next row is on its way while this one's sums are formed
+#pragma unroll
+      for (int p = 0; p < NV; ++p) next[p] = load_piece<T, ALIGNED>(x + (long long)(t + step) * xs, p * group + in_group, d);
+    float2 s2 = both(0.f);
+#pragma unroll
+    for (int p = 0; p < NV; ++p)
+#pragma unroll
+      for (int e = 0; e < H; ++e) s2 = add2(s2, v[p][e]);
+    const float s = warp_sum_f(s2.x + s2.y);
+    float mu = s * inv_own;
+    float2 q2 = both(0.f);
+#pragma unroll
+    for (int p = 0; p < NV; ++p) {
+      const int c = (p * group + in_group) * V;
+      if (ALIGNED && c >= d) continue;
+#pragma unroll
+      for (int e = 0; e < H; ++e) {
+        float2 o = add2(v[p][e], both(-mu));
+        if (!ALIGNED) {
+          if (c + 2 * e >= d) o.x = 0.f;
+          if (c + 2 * e + 1 >= d) o.y = 0.f;
+        }
+        q2 = fma2(o, o, q2);
       }
-      q2 = fma2(o, o, q2);
     }
-  }
-  float q = warp_sum_f(q2.x + q2.y);
-  const int warps = group / 32;
-  if (warps > 1) {
-    if (lane == 0) red[threadIdx.x / 32] = make_float2(s, q);
-    group_sync(group);
-    const float2 o = lane < warps ? red[which * warps + lane] : both(0.f);
-    mu = warp_sum_f(o.x) * inv_d;
-    const int n = lane < warps ? columns(lane) : 0;
-    const float near = __fdividef(o.x, (float)max(1, n)), off = near - mu;
-    q = warp_sum_f(fmaf((float)n * off, off, o.y));
-  } else {
-    // M2 about the mean from M2 about a number near it
-    const float m = s * inv_d, off = m - mu;
-    q = fmaf((float)(-d) * off, off, q);
-    mu = m;
-  }
-  const float r = 1.f / sqrtf(q * inv_d + eps);
-  T* yr = y + (long long)t * ys;
+    float q = warp_sum_f(q2.x + q2.y);
+    if (warps > 1) {
+      float2* mine = red[turn] + threadIdx.y * warps;
+      if (lane == 0) mine[threadIdx.x / 32] = make_float2(s, q);
+      group_sync();
+      const float2 o = (lane & 15) < warps ? mine[lane & 15] : both(0.f);      // both halves of the warp alike
+      mu = half_warp_sum(o.x) * inv_d;
+      const float off = o.x * inv_lane - mu;
+      q = half_warp_sum(fmaf(n_lane * off, off, o.y));
+    }
+    const float r = rsqrtf(fmaf(q, inv_d, eps));
+    T* yr = y + (long long)t * ys;
 #pragma unroll
-  for (int p = 0; p < NV; ++p) {
-    const int i = p * group + in_group;
-    float2 wf[H], bf[H];
-    load_params<P, H, ALIGNED>(w, i, d, 1.f, wf);
-    load_params<P, H, ALIGNED>(b, i, d, 0.f, bf);
+    for (int p = 0; p < NV; ++p) {
 #pragma unroll
-    for (int e = 0; e < H; ++e) v[p][e] = fma2(mul2(add2(v[p][e], both(-mu)), both(r)), wf[e], bf[e]);
-    store_piece<T, ALIGNED>(yr, i, d, pack<T>(v[p]));
-  }
-  if (in_group == 0) {
-    if (mean) mean[t] = mu;
-    if (rstd) rstd[t] = r;
+      for (int e = 0; e < H; ++e) v[p][e] = fma2(mul2(add2(v[p][e], both(-mu)), both(r)), wf[p][e], bf[p][e]);
+      store_piece<T, ALIGNED>(yr, p * group + in_group, d, pack<T>(v[p]));
+    }
+    if (in_group == 0) {
+      if (mean) mean[t] = mu;
+      if (rstd) rstd[t] = r;
+    }
   }
 }
 
@@ -158,11 +160,11 @@ norm_rows_kernel(const T* x, long long xs, int rows, int d, float inv_d, const P
 template <typename T, typename P, int NV, bool ALIGNED>
 __global__ void __launch_bounds__(1024)
 norm_grad_rows_kernel(const T* dy, long long dys, const T* x, long long xs, const float* mean, const float* rstd, int rows, int d,
-                      float inv_d, const P* w, T* dx, long long dxs, float* part, int group) {
+                      float inv_d, const P* w, T* dx, long long dxs, float* part) {
   constexpr int V = Piece<T>::V, H = V / 2;
   __shared__ float2 red[2][32];      // used in turn: one half may still be read by slower warps
-  const int per_cta = blockDim.x / group, which = threadIdx.x / group, in_group = threadIdx.x - which * group, warps = group / 32;
-  const int lane = threadIdx.x & 31;
+  const int group = blockDim.x, per_cta = blockDim.y, which = threadIdx.y, in_group = threadIdx.x, lane = threadIdx.x & 31;
+  const int warps = group / 32;
   float2 aw[NV][H], ab[NV][H];
 #pragma unroll
   for (int p = 0; p < NV; ++p)
@@ -215,9 +217,10 @@ norm_grad_rows_kernel(const T* dy, long long dys, const T* x, long long xs, cons
     }
     float s1 = warp_sum_f(a2.x + a2.y), s2 = warp_sum_f(b2.x + b2.y);
     if (warps > 1) {
-      if (lane == 0) red[turn][threadIdx.x / 32] = make_float2(s1, s2);
-      group_sync(group);
-      const float2 o = lane < warps ? red[turn][which * warps + lane] : both(0.f);
+      float2* mine = red[turn] + which * warps;
+      if (lane == 0) mine[threadIdx.x / 32] = make_float2(s1, s2);
+      group_sync();
+      const float2 o = lane < warps ? mine[lane] : both(0.f);
       s1 = warp_sum_f(o.x);
       s2 = warp_sum_f(o.y);
     }
@@ -251,7 +254,7 @@ norm_grad_rows_kernel(const T* dy, long long dys, const T* x, long long xs, cons
   }
   __syncthreads();
   if (per_cta > 1)
-    for (int c = threadIdx.x; c < 2 * d; c += blockDim.x) pw[c] = cols[c];
+    for (int c = which * group + in_group; c < 2 * d; c += group * per_cta) pw[c] = cols[c];
 }
 
 // Rows wider than the registers take: one CTA per row, the row read again (from L2) for each of its sums.
@@ -335,20 +338,19 @@ norm_grad_sum_kernel(const float* part, int parts, int d, float* dw, float* db) 
   }
 }
 
-// CTAs of the gradient's walk, each of which leaves a partial sum: as many as run at once with 64 registers a thread.
-constexpr int kNormGradMost = 2;     // pieces a thread has of float32 rows; 16-bit rows have one
-inline NormShape norm_grad_shape(int d, int size) { return norm_shape(d, 16 / size, size == 4 ? kNormGradMost : 1); }
-inline int norm_grad_grid(size_t rows, const NormShape& s, int sms) {
+// CTAs of a walk: as many as run at once.  Of the gradient's, each leaves a partial sum.
+constexpr int kNormGradThreadsPerSm = 1024;
+inline NormShape norm_grad_shape(int d, int size) { return norm_shape(d, 16 / size, size == 4 ? 2 : 1, 1024); }
+inline int norm_grid(size_t rows, const NormShape& s, int sms, int threads_per_sm) {
   if (!s.group) return (int)std::min<size_t>(rows, (size_t)sms * 4);
-  return (int)std::min<size_t>((rows + s.per_cta - 1) / s.per_cta, (size_t)sms * (1024 / s.threads()));
+  return (int)std::min<size_t>((rows + s.per_cta - 1) / s.per_cta, (size_t)sms * std::max(1, threads_per_sm / s.threads()));
 }
 
 template <typename T, typename P, bool ALIGNED>
-int norm_launch(const NormShape& s, const T* x, long long xs, int rows, int d, const P* w, const P* b, float eps, T* y,
+int norm_launch(const NormShape& s, int grid, const T* x, long long xs, int rows, int d, const P* w, const P* b, float eps, T* y,
                 long long ys, float* mean, float* rstd, cudaStream_t stream) {
-  auto fn = s.nv == 1 ? norm_rows_kernel<T, P, 1, ALIGNED> : s.nv == 2 ? norm_rows_kernel<T, P, 2, ALIGNED>
-                                                                       : norm_rows_kernel<T, P, 4, ALIGNED>;
-  fn<<<(rows + s.per_cta - 1) / s.per_cta, s.threads(), 0, stream>>>(x, xs, rows, d, 1.f / (float)d, w, b, eps, y, ys, mean, rstd, s.group);
+  auto fn = s.nv == 1 ? norm_rows_kernel<T, P, 1, ALIGNED> : norm_rows_kernel<T, P, 2, ALIGNED>;
+  fn<<<grid, dim3(s.group, s.per_cta), 0, stream>>>(x, xs, rows, d, 1.f / (float)d, w, b, eps, y, ys, mean, rstd);
   KM_CUDA(cudaGetLastError());
   return KM_OK;
 }
@@ -361,7 +363,7 @@ int norm_grad_launch(const NormShape& s, int grid, const T* dy, long long dys, c
     if (s.nv == 2) fn = norm_grad_rows_kernel<T, P, 2, ALIGNED>;
   // several groups a CTA: at most 1024 columns, 8 KB
   const size_t smem = part && s.per_cta > 1 ? (size_t)2 * d * sizeof(float) : 0;
-  fn<<<grid, s.threads(), smem, stream>>>(dy, dys, x, xs, mean, rstd, rows, d, 1.f / (float)d, w, dx, dxs, part, s.group);
+  fn<<<grid, dim3(s.group, s.per_cta), smem, stream>>>(dy, dys, x, xs, mean, rstd, rows, d, 1.f / (float)d, w, dx, dxs, part);
   KM_CUDA(cudaGetLastError());
   return KM_OK;
 }

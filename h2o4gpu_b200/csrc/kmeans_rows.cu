@@ -41,7 +41,10 @@ int layer_norm(int dtype, const void* x, long long xs, size_t rows, size_t cols,
       !aligned(mean, 4) || !aligned(rstd, 4))
     KM_FAIL(KM_EINVAL, "kmeans_layer_norm: bad argument");
   const int d = (int)cols;
-  const NormShape shape = norm_shape(d, 16 / size, 4);
+  int sms = 0;
+  KM_TRY(sm_count(&sms));
+  const NormShape shape = norm_shape(d, 16 / size, 2, kNormMaxThreads);
+  const int grid = norm_grid(rows, shape, sms, kNormThreadsPerSm);
   const bool al = rows_aligned(x, xs, rows, cols, size) && rows_aligned(y, ys, rows, cols, size) && aligned(weight, 16) &&
                   aligned(bias, 16);
   int rc = KM_OK;
@@ -54,16 +57,16 @@ int layer_norm(int dtype, const void* x, long long xs, size_t rows, size_t cols,
         norm_wide_kernel<T, P><<<(unsigned)rows, kNormThreads, 0, stream>>>(xp, xs, d, wp, bp, (float)eps, yp, ys, mean, rstd);
         KM_CUDA(cudaGetLastError());
       } else if (al) {
-        rc = norm_launch<T, P, true>(shape, xp, xs, (int)rows, d, wp, bp, (float)eps, yp, ys, mean, rstd, stream);
+        rc = norm_launch<T, P, true>(shape, grid, xp, xs, (int)rows, d, wp, bp, (float)eps, yp, ys, mean, rstd, stream);
       } else {
-        rc = norm_launch<T, P, false>(shape, xp, xs, (int)rows, d, wp, bp, (float)eps, yp, ys, mean, rstd, stream);
+        rc = norm_launch<T, P, false>(shape, grid, xp, xs, (int)rows, d, wp, bp, (float)eps, yp, ys, mean, rstd, stream);
       }));
   return rc;
 }
 
 // Partial sums of the gradient's walk over rows of `size`-byte elements.
 int norm_grad_parts(size_t rows, size_t cols, int size, int sms) {
-  return norm_grad_grid(rows, norm_grad_shape((int)cols, size), sms);
+  return norm_grid(rows, norm_grad_shape((int)cols, size), sms, kNormGradThreadsPerSm);
 }
 
 int layer_norm_grad_workspace(size_t rows, size_t cols, size_t* bytes) {
