@@ -3,6 +3,7 @@
 
 #include <cuda_bf16.h>
 
+#include <atomic>
 #include <cmath>
 #include <exception>
 
@@ -83,6 +84,22 @@ inline int sm_count(int* out) {
   *out = count[dev];
   return KM_OK;
 }
+
+// CTAs of a kernel that fit a multiprocessor at once, asked once per number of threads.
+struct ResidentCtas {
+  std::atomic<int> known[33] = {};     // by warps
+  template <typename F>
+  int get(F fn, int threads, int* out) {
+    std::atomic<int>& k = known[threads / 32];
+    *out = k.load(std::memory_order_relaxed);
+    if (*out == 0) {
+      KM_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(out, fn, threads, 0));
+      *out = std::max(1, *out);
+      k.store(*out, std::memory_order_relaxed);
+    }
+    return KM_OK;
+  }
+};
 
 // What a C entry point runs: nothing may leave it but a code.
 template <typename F>

@@ -11,16 +11,14 @@ namespace rows {
 
 constexpr int kNormThreads = 256;   // of the kernels for wide rows
 
-// Weights or biases of the columns of piece i (2 H of them), `none` without them.  They stay in L1 from row to row.
+// Weights or biases of the columns of piece i (2 H of them), `none` behind the row's end.  They stay in L1 from row to row.
 template <typename P, int H, bool ALIGNED>
-__device__ __forceinline__ void load_params(const P* w, int i, int d, float none, float2 (&f)[H]) {
+__device__ __forceinline__ void load_params(const P* w, int i, int d, bool inside, float none, float2 (&f)[H]) {
   constexpr int V = 2 * H;
   const int c = i * V;
-  if (w == nullptr || c >= d) {
 #pragma unroll
-    for (int e = 0; e < H; ++e) f[e] = both(none);
-    return;
-  }
+  for (int e = 0; e < H; ++e) f[e] = both(none);
+  if (!inside) return;
   if (ALIGNED) {      // of whole pieces
     constexpr int PV = Piece<P>::V;
 #pragma unroll
@@ -39,6 +37,21 @@ __device__ __forceinline__ void load_params(const P* w, int i, int d, float none
   }
 }
 
+// Pieces of a row that a lane holds: `have` of them lie in the row, the others are never loaded and stay zero (a load that
+// fills in zeros, addresses that are formed for every piece and row cost more instructions than the sums).
+template <typename T, int NV, bool ALIGNED>
+__device__ __forceinline__ void load_pieces(const T* row, int first, int have, int d, Piece<T> (&p)[NV]) {
+  const uint4* q = reinterpret_cast<const uint4*>(row) + first;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    if (ALIGNED) {
+      if (i < have) p[i].q = q[i * 32];
+    } else {
+      p[i] = load_piece<T, false>(row, first + i * 32, d);
+    }
+  }
+}
+
 // How a row is spread: `group` threads (whole warps) take it, NV pieces of 16 bytes each; `per_cta` groups share a CTA.  A group walks
 // through the rows with the grid, so that a thread always has the same columns.
 struct NormShape {
@@ -47,15 +60,15 @@ struct NormShape {
   int per_cta = 1;
   int threads() const { return group * per_cta; }
 };
-// One warp while it can take the row (no barrier), else `most` pieces a thread.
-inline NormShape norm_shape(int d, int v, int most, int max_threads) {
-  const int pieces = (d + v - 1) / v;
+// As few warps as can hold the row, 32 columns a lane at most: what a row costs besides its values - two sums over the lanes, the
+// joining of the warps, addresses - is paid per warp.
+inline NormShape norm_shape(int d, int size, int max_threads) {
+  const int v = 16 / size, pieces = (d + v - 1) / v, most = 32 / v, warps = (pieces + 32 * most - 1) / (32 * most);
   NormShape s;
-  const auto warps = [&](int nv) { return (pieces + 32 * nv - 1) / (32 * nv); };
-  s.nv = pieces <= 32 ? 1 : most;
-  if (32 * warps(s.nv) > max_threads) return s;
-  s.group = 32 * warps(s.nv);
-  s.per_cta = std::max(1, 256 / s.group);
+  s.nv = (pieces + 32 * warps - 1) / (32 * warps);
+  if (32 * warps > max_threads) return s;
+  s.group = 32 * warps;
+  s.per_cta = std::max(1, 128 / s.group);
   return s;
 }
 
@@ -66,47 +79,33 @@ __device__ __forceinline__ void group_sync() {
 
 // Mean and sum of squared differences from it.  Each warp takes them of its own columns first - its mean, then the differences - and the
 // warps join by  M2 = sum of M2_w + n_w (mean_w - mean)^2:  no cancellation as in E x^2 - (E x)^2, and one barrier instead of two.
-// A row costs some 8 operations a value on pipes that a memory-bound kernel fills to two thirds, so weights and biases stay in
-// registers (as float32 pairs: unpacking them again for every row was a tenth of the instructions), and the columns' counts are
-// taken before the walk.
 constexpr int kNormMaxThreads = 512;       // a row's group
-constexpr int kNormRegs = 80;              // so that 24 warps fit a processor
-constexpr int kNormThreadsPerSm = 768;
 template <typename T, typename P, int NV, bool ALIGNED>
-__global__ void __maxnreg__(kNormRegs)
+__global__ void __launch_bounds__(kNormMaxThreads)
 norm_rows_kernel(const T* x, long long xs, int rows, int d, float inv_d, const P* w, const P* b, float eps, T* y, long long ys,
                  float* mean, float* rstd) {
   constexpr int V = Piece<T>::V, H = V / 2;
-  __shared__ float2 red[2][32];      // used in turn: one half may still be read by slower warps
-  const int group = blockDim.x, in_group = threadIdx.x, lane = threadIdx.x & 31, warps = group / 32;
-  // the columns that warp `i` of the group has
-  const auto columns = [&](int i) {
-    int n = 0;
-#pragma unroll
-    for (int p = 0; p < NV; ++p) n += max(0, min(32 * V, d - (p * group + i * 32) * V));
-    return (float)n;
-  };
+  __shared__ float2 red[2][16];      // used in turn: one half may still be read by slower warps
+  const int in_group = threadIdx.x, lane = threadIdx.x & 31, warps = blockDim.x / 32;
+  // warp i of the group has the 32 NV pieces from i * 32 NV on, each lane every 32nd of them
+  const auto columns = [&](int i) { return (float)max(0, min(32 * NV * V, d - i * 32 * NV * V)); };
+  const int first = in_group / 32 * (32 * NV) + lane;
+  const int have = min(NV, max(0, ((d + V - 1) / V - first + 31) / 32));
   const float n_own = columns(in_group / 32), n_lane = (lane & 15) < warps ? columns(lane & 15) : 0.f;
   const float inv_own = n_own > 0.f ? 1.f / n_own : 0.f, inv_lane = n_lane > 0.f ? 1.f / n_lane : 0.f;
-  float2 wf[NV][H], bf[NV][H];
-#pragma unroll
-  for (int p = 0; p < NV; ++p) {
-    load_params<P, H, ALIGNED>(w, p * group + in_group, d, 1.f, wf[p]);
-    load_params<P, H, ALIGNED>(b, p * group + in_group, d, 0.f, bf[p]);
-  }
   const int step = gridDim.x * blockDim.y;
   int t = blockIdx.x * blockDim.y + threadIdx.y, turn = 0;
-  Piece<T> next[NV];
-  if (t < rows)
+  // the next row is on its way into one buffer while the other one's sums are formed
+  Piece<T> one[NV], two[NV];
 #pragma unroll
-    for (int p = 0; p < NV; ++p) next[p] = load_piece<T, ALIGNED>(x + (long long)t * xs, p * group + in_group, d);
-  for (; t < rows; t += step, turn ^= 1) {
+  for (int p = 0; p < NV; ++p) one[p].q = two[p].q = make_uint4(0u, 0u, 0u, 0u);
+  const auto load = [&](int row, Piece<T>(&p)[NV]) {
+    if (row < rows) load_pieces<T, NV, ALIGNED>(x + (long long)row * xs, first, have, d, p);
+  };
+  const auto norm = [&](const Piece<T>(&raw)[NV]) {
     float2 v[NV][H];
 #pragma unroll
-    for (int p = 0; p < NV; ++p) unpack(next[p], v[p]);
-    if (t + step < rows)      // the next row is on its way while this one's sums are formed
-#pragma unroll
-      for (int p = 0; p < NV; ++p) next[p] = load_piece<T, ALIGNED>(x + (long long)(t + step) * xs, p * group + in_group, d);
+    for (int p = 0; p < NV; ++p) unpack(raw[p], v[p]);
     float2 s2 = both(0.f);
 #pragma unroll
     for (int p = 0; p < NV; ++p)
@@ -117,8 +116,8 @@ norm_rows_kernel(const T* x, long long xs, int rows, int d, float inv_d, const P
     float2 q2 = both(0.f);
 #pragma unroll
     for (int p = 0; p < NV; ++p) {
-      const int c = (p * group + in_group) * V;
-      if (ALIGNED && c >= d) continue;
+      if (ALIGNED && p >= have) continue;
+      const int c = (first + p * 32) * V;
 #pragma unroll
       for (int e = 0; e < H; ++e) {
         float2 o = add2(v[p][e], both(-mu));
@@ -132,7 +131,7 @@ norm_rows_kernel(const T* x, long long xs, int rows, int d, float inv_d, const P
     float q = warp_sum_f(q2.x + q2.y);
     if (warps > 1) {
       float2* mine = red[turn] + threadIdx.y * warps;
-      if (lane == 0) mine[threadIdx.x / 32] = make_float2(s, q);
+      if (lane == 0) mine[in_group / 32] = make_float2(s, q);
       group_sync();
       const float2 o = (lane & 15) < warps ? mine[lane & 15] : both(0.f);      // both halves of the warp alike
       mu = half_warp_sum(o.x) * inv_d;
@@ -141,97 +140,146 @@ norm_rows_kernel(const T* x, long long xs, int rows, int d, float inv_d, const P
     }
     const float r = rsqrtf(fmaf(q, inv_d, eps));
     T* yr = y + (long long)t * ys;
+    const auto finish = [&](auto with_w, auto with_b) {
+      uint4* out = reinterpret_cast<uint4*>(yr) + first;
 #pragma unroll
-    for (int p = 0; p < NV; ++p) {
+      for (int p = 0; p < NV; ++p) {
+        const int i = first + p * 32;
+        float2 wf[H], bf[H];
+        if (with_w()) load_params<P, H, ALIGNED>(w, i, d, p < have, 1.f, wf);
+        if (with_b()) load_params<P, H, ALIGNED>(b, i, d, p < have, 0.f, bf);
 #pragma unroll
-      for (int e = 0; e < H; ++e) v[p][e] = fma2(mul2(add2(v[p][e], both(-mu)), both(r)), wf[p][e], bf[p][e]);
-      store_piece<T, ALIGNED>(yr, p * group + in_group, d, pack<T>(v[p]));
-    }
+        for (int e = 0; e < H; ++e) {
+          float2 o = mul2(add2(v[p][e], both(-mu)), both(r));
+          if (with_w() && with_b()) o = fma2(o, wf[e], bf[e]);
+          else if (with_w()) o = mul2(o, wf[e]);
+          else if (with_b()) o = add2(o, bf[e]);
+          v[p][e] = o;
+        }
+        if (ALIGNED) {
+          if (p < have) out[p * 32] = pack<T>(v[p]).q;
+        } else {
+          store_piece<T, false>(yr, i, d, pack<T>(v[p]));
+        }
+      }
+    };
+    using std::integral_constant;
+    if (w && b) finish(integral_constant<bool, true>(), integral_constant<bool, true>());
+    else if (w) finish(integral_constant<bool, true>(), integral_constant<bool, false>());
+    else if (b) finish(integral_constant<bool, false>(), integral_constant<bool, true>());
+    else finish(integral_constant<bool, false>(), integral_constant<bool, false>());
     if (in_group == 0) {
       if (mean) mean[t] = mu;
       if (rstd) rstd[t] = r;
     }
+    t += step;
+    turn ^= 1;
+  };
+  load(t, one);
+  while (t < rows) {
+    load(t + step, two);
+    norm(one);
+    if (t >= rows) break;
+    load(t + step, one);
+    norm(two);
   }
 }
 
 // The gradient.  A group walks through the rows with the grid, so that a thread always has the same columns, and adds their dy xh
 // and dy; the CTA joins its groups in their order and leaves its sums in part[CTA] (dw then db, d each), which
 // norm_grad_sum_kernel adds up in the CTAs' order.
+constexpr int kNormGradMaxThreads = 256;
 template <typename T, typename P, int NV, bool ALIGNED>
-__global__ void __launch_bounds__(1024)
+__global__ void __launch_bounds__(kNormGradMaxThreads)
 norm_grad_rows_kernel(const T* dy, long long dys, const T* x, long long xs, const float* mean, const float* rstd, int rows, int d,
                       float inv_d, const P* w, T* dx, long long dxs, float* part) {
   constexpr int V = Piece<T>::V, H = V / 2;
-  __shared__ float2 red[2][32];      // used in turn: one half may still be read by slower warps
+  __shared__ float2 red[2][8];      // used in turn: one half may still be read by slower warps
   const int group = blockDim.x, per_cta = blockDim.y, which = threadIdx.y, in_group = threadIdx.x, lane = threadIdx.x & 31;
   const int warps = group / 32;
+  const int first = in_group / 32 * (32 * NV) + lane;      // as in norm_rows_kernel
+  const int have = min(NV, max(0, ((d + V - 1) / V - first + 31) / 32));
   float2 aw[NV][H], ab[NV][H];
+  struct Row {
+    Piece<T> x[NV], g[NV];
+    float mu, r;
+  };
+  Row one, two;      // the next row is on its way into one while the other one's sums are formed
 #pragma unroll
-  for (int p = 0; p < NV; ++p)
+  for (int p = 0; p < NV; ++p) {
+    one.x[p].q = one.g[p].q = two.x[p].q = two.g[p].q = make_uint4(0u, 0u, 0u, 0u);
 #pragma unroll
     for (int e = 0; e < H; ++e) aw[p][e] = ab[p][e] = both(0.f);
+  }
   const int step = gridDim.x * per_cta;
   int t = blockIdx.x * per_cta + which, turn = 0;
-  Piece<T> nx[NV], ng[NV];
-  float nmu = 0.f, nr = 0.f;
-  if (t < rows) {
-#pragma unroll
-    for (int p = 0; p < NV; ++p) {
-      nx[p] = load_piece<T, ALIGNED>(x + (long long)t * xs, p * group + in_group, d);
-      ng[p] = load_piece<T, ALIGNED>(dy + (long long)t * dys, p * group + in_group, d);
-    }
-    nmu = mean[t];
-    nr = rstd[t];
-  }
-  for (; t < rows; t += step, turn ^= 1) {
-    const float mu = nmu, r = nr;
+  const auto load = [&](int row, Row& to) {
+    if (row >= rows) return;
+    load_pieces<T, NV, ALIGNED>(x + (long long)row * xs, first, have, d, to.x);
+    load_pieces<T, NV, ALIGNED>(dy + (long long)row * dys, first, have, d, to.g);
+    to.mu = mean[row];
+    to.r = rstd[row];
+  };
+  const auto grad = [&](const Row& row) {
+    const float r = row.r;
+    const float2 rr = both(r), off = both(-row.mu * r);      // xh = x r - mu r: this rounding is no larger than the stored mean's
     float2 xh[NV][H], g[NV][H];
 #pragma unroll
     for (int p = 0; p < NV; ++p) {
-      unpack(nx[p], xh[p]);
-      unpack(ng[p], g[p]);
-    }
-    if (t + step < rows) {     // the next row is on its way while this one's sums are formed
-#pragma unroll
-      for (int p = 0; p < NV; ++p) {
-        nx[p] = load_piece<T, ALIGNED>(x + (long long)(t + step) * xs, p * group + in_group, d);
-        ng[p] = load_piece<T, ALIGNED>(dy + (long long)(t + step) * dys, p * group + in_group, d);
-      }
-      nmu = mean[t + step];
-      nr = rstd[t + step];
+      unpack(row.x[p], xh[p]);
+      unpack(row.g[p], g[p]);
     }
     float2 a2 = both(0.f), b2 = both(0.f);
+    const auto sums = [&](auto with_w) {
 #pragma unroll
-    for (int p = 0; p < NV; ++p) {
-      float2 wf[H];
-      load_params<P, H, ALIGNED>(w, p * group + in_group, d, 1.f, wf);
+      for (int p = 0; p < NV; ++p) {
+        float2 wf[H];
+        if (with_w()) load_params<P, H, ALIGNED>(w, first + p * 32, d, p < have, 1.f, wf);
 #pragma unroll
-      for (int e = 0; e < H; ++e) {
-        xh[p][e] = mul2(add2(xh[p][e], both(-mu)), both(r));     // behind the row's end g is zero
-        aw[p][e] = fma2(g[p][e], xh[p][e], aw[p][e]);
-        ab[p][e] = add2(ab[p][e], g[p][e]);
-        g[p][e] = mul2(g[p][e], wf[e]);
-        a2 = add2(a2, g[p][e]);
-        b2 = fma2(g[p][e], xh[p][e], b2);
+        for (int e = 0; e < H; ++e) {
+          xh[p][e] = fma2(xh[p][e], rr, off);     // behind the row's end g is zero
+          aw[p][e] = fma2(g[p][e], xh[p][e], aw[p][e]);
+          ab[p][e] = add2(ab[p][e], g[p][e]);
+          if (with_w()) g[p][e] = mul2(g[p][e], wf[e]);
+          a2 = add2(a2, g[p][e]);
+          b2 = fma2(g[p][e], xh[p][e], b2);
+        }
       }
-    }
+    };
+    if (w) sums(std::integral_constant<bool, true>());
+    else sums(std::integral_constant<bool, false>());
     float s1 = warp_sum_f(a2.x + a2.y), s2 = warp_sum_f(b2.x + b2.y);
     if (warps > 1) {
       float2* mine = red[turn] + which * warps;
-      if (lane == 0) mine[threadIdx.x / 32] = make_float2(s1, s2);
+      if (lane == 0) mine[in_group / 32] = make_float2(s1, s2);
       group_sync();
-      const float2 o = lane < warps ? mine[lane] : both(0.f);
-      s1 = warp_sum_f(o.x);
-      s2 = warp_sum_f(o.y);
+      const float2 o = (lane & 15) < warps ? mine[lane & 15] : both(0.f);
+      s1 = half_warp_sum(o.x);
+      s2 = half_warp_sum(o.y);
     }
-    const float2 m1 = both(-s1 * inv_d), m2 = both(-s2 * inv_d);
+    const float2 m1 = both(-r * (s1 * inv_d)), m2 = both(-r * (s2 * inv_d));
     T* dr = dx + (long long)t * dxs;
+    uint4* out = reinterpret_cast<uint4*>(dr) + first;
 #pragma unroll
     for (int p = 0; p < NV; ++p) {
 #pragma unroll
-      for (int e = 0; e < H; ++e) g[p][e] = mul2(both(r), fma2(xh[p][e], m2, add2(g[p][e], m1)));
-      store_piece<T, ALIGNED>(dr, p * group + in_group, d, pack<T>(g[p]));
+      for (int e = 0; e < H; ++e) g[p][e] = fma2(xh[p][e], m2, fma2(g[p][e], rr, m1));
+      if (ALIGNED) {
+        if (p < have) out[p * 32] = pack<T>(g[p]).q;
+      } else {
+        store_piece<T, false>(dr, first + p * 32, d, pack<T>(g[p]));
+      }
     }
+    t += step;
+    turn ^= 1;
+  };
+  load(t, one);
+  while (t < rows) {
+    load(t + step, two);
+    grad(one);
+    if (t >= rows) break;
+    load(t + step, one);
+    grad(two);
   }
   if (!part) return;
   extern __shared__ float joined[];     // dw then db of the CTA, d each
@@ -244,7 +292,7 @@ norm_grad_rows_kernel(const T* dy, long long dys, const T* x, long long xs, cons
       for (int p = 0; p < NV; ++p)
 #pragma unroll
         for (int e = 0; e < V; ++e) {
-          const int c = (p * group + in_group) * V + e;
+          const int c = (first + p * 32) * V + e;
           if (c < d) {
             const float sw = e & 1 ? aw[p][e / 2].y : aw[p][e / 2].x, sb = e & 1 ? ab[p][e / 2].y : ab[p][e / 2].x;
             cols[c] = grp ? cols[c] + sw : sw;
@@ -338,34 +386,61 @@ norm_grad_sum_kernel(const float* part, int parts, int d, float* dw, float* db) 
   }
 }
 
-// CTAs of a walk: as many as run at once.  Of the gradient's, each leaves a partial sum.
-constexpr int kNormGradThreadsPerSm = 1024;
-inline NormShape norm_grad_shape(int d, int size) { return norm_shape(d, 16 / size, size == 4 ? 2 : 1, 1024); }
+// CTAs of a walk: as many as run at once (per processor, from the kernel's registers).  Of the gradient's, each leaves a partial sum; their
+// number must not depend on more than the sizes and the element size, which is all that the workspace is asked for.
+constexpr int kNormGradThreadsPerSm = 256;
+inline NormShape norm_grad_shape(int d, int size) { return norm_shape(d, size, kNormGradMaxThreads); }
 inline int norm_grid(size_t rows, const NormShape& s, int sms, int threads_per_sm) {
   if (!s.group) return (int)std::min<size_t>(rows, (size_t)sms * 4);
   return (int)std::min<size_t>((rows + s.per_cta - 1) / s.per_cta, (size_t)sms * std::max(1, threads_per_sm / s.threads()));
 }
 
+// f(NV) with the number of pieces as a constant.
+template <typename T, typename F>
+int with_pieces(int nv, F&& f) {
+  using std::integral_constant;
+  switch (nv) {
+    case 1: return f(integral_constant<int, 1>());
+    case 2: return f(integral_constant<int, 2>());
+    case 3: return f(integral_constant<int, 3>());
+    case 4: return f(integral_constant<int, 4>());
+  }
+  if constexpr (sizeof(T) == 4) switch (nv) {
+    case 5: return f(integral_constant<int, 5>());
+    case 6: return f(integral_constant<int, 6>());
+    case 7: return f(integral_constant<int, 7>());
+    case 8: return f(integral_constant<int, 8>());
+  }
+  return KM_EINVAL;
+}
+
 template <typename T, typename P, bool ALIGNED>
-int norm_launch(const NormShape& s, int grid, const T* x, long long xs, int rows, int d, const P* w, const P* b, float eps, T* y,
+int norm_launch(const NormShape& s, int sms, const T* x, long long xs, int rows, int d, const P* w, const P* b, float eps, T* y,
                 long long ys, float* mean, float* rstd, cudaStream_t stream) {
-  auto fn = s.nv == 1 ? norm_rows_kernel<T, P, 1, ALIGNED> : norm_rows_kernel<T, P, 2, ALIGNED>;
-  fn<<<grid, dim3(s.group, s.per_cta), 0, stream>>>(x, xs, rows, d, 1.f / (float)d, w, b, eps, y, ys, mean, rstd);
-  KM_CUDA(cudaGetLastError());
-  return KM_OK;
+  return with_pieces<T>(s.nv, [&](auto nv) -> int {
+    static ResidentCtas resident;
+    const auto fn = norm_rows_kernel<T, P, nv(), ALIGNED>;
+    int per_sm = 0;
+    KM_TRY(resident.get(fn, s.threads(), &per_sm));
+    const int grid = norm_grid(rows, s, sms, per_sm * s.threads());
+    fn<<<grid, dim3(s.group, s.per_cta), 0, stream>>>(x, xs, rows, d, 1.f / (float)d, w, b, eps, y,
+                                                                                        ys, mean, rstd);
+    KM_CUDA(cudaGetLastError());
+    return KM_OK;
+  });
 }
 
 template <typename T, typename P, bool ALIGNED>
 int norm_grad_launch(const NormShape& s, int grid, const T* dy, long long dys, const T* x, long long xs, const float* mean,
                      const float* rstd, int rows, int d, const P* w, T* dx, long long dxs, float* part, cudaStream_t stream) {
-  auto fn = norm_grad_rows_kernel<T, P, 1, ALIGNED>;
-  if constexpr (sizeof(T) == 4)
-    if (s.nv == 2) fn = norm_grad_rows_kernel<T, P, 2, ALIGNED>;
-  // several groups a CTA: at most 1024 columns, 8 KB
-  const size_t smem = part && s.per_cta > 1 ? (size_t)2 * d * sizeof(float) : 0;
-  fn<<<grid, dim3(s.group, s.per_cta), smem, stream>>>(dy, dys, x, xs, mean, rstd, rows, d, 1.f / (float)d, w, dx, dxs, part);
-  KM_CUDA(cudaGetLastError());
-  return KM_OK;
+  return with_pieces<T>(s.nv, [&](auto nv) -> int {
+    // several groups a CTA: at most 2048 columns, 16 KB
+    const size_t smem = part && s.per_cta > 1 ? (size_t)2 * d * sizeof(float) : 0;
+    norm_grad_rows_kernel<T, P, nv(), ALIGNED><<<grid, dim3(s.group, s.per_cta), smem, stream>>>(
+        dy, dys, x, xs, mean, rstd, rows, d, 1.f / (float)d, w, dx, dxs, part);
+    KM_CUDA(cudaGetLastError());
+    return KM_OK;
+  });
 }
 
 }  // namespace rows

@@ -43,8 +43,7 @@ int layer_norm(int dtype, const void* x, long long xs, size_t rows, size_t cols,
   const int d = (int)cols;
   int sms = 0;
   KM_TRY(sm_count(&sms));
-  const NormShape shape = norm_shape(d, 16 / size, 2, kNormMaxThreads);
-  const int grid = norm_grid(rows, shape, sms, kNormThreadsPerSm);
+  const NormShape shape = norm_shape(d, size, kNormMaxThreads);
   const bool al = rows_aligned(x, xs, rows, cols, size) && rows_aligned(y, ys, rows, cols, size) && aligned(weight, 16) &&
                   aligned(bias, 16);
   int rc = KM_OK;
@@ -57,9 +56,9 @@ int layer_norm(int dtype, const void* x, long long xs, size_t rows, size_t cols,
         norm_wide_kernel<T, P><<<(unsigned)rows, kNormThreads, 0, stream>>>(xp, xs, d, wp, bp, (float)eps, yp, ys, mean, rstd);
         KM_CUDA(cudaGetLastError());
       } else if (al) {
-        rc = norm_launch<T, P, true>(shape, grid, xp, xs, (int)rows, d, wp, bp, (float)eps, yp, ys, mean, rstd, stream);
+        rc = norm_launch<T, P, true>(shape, sms, xp, xs, (int)rows, d, wp, bp, (float)eps, yp, ys, mean, rstd, stream);
       } else {
-        rc = norm_launch<T, P, false>(shape, grid, xp, xs, (int)rows, d, wp, bp, (float)eps, yp, ys, mean, rstd, stream);
+        rc = norm_launch<T, P, false>(shape, sms, xp, xs, (int)rows, d, wp, bp, (float)eps, yp, ys, mean, rstd, stream);
       }));
   return rc;
 }
