@@ -188,39 +188,57 @@ norm_rows_kernel(const T* x, long long xs, int rows, int d, float inv_d, const P
 // The gradient.  A group walks through the rows with the grid, so that a thread always has the same columns, and adds their dy xh
 // and dy; the CTA joins its groups in their order and leaves its sums in part[CTA] (dw then db, d each), which
 // norm_grad_sum_kernel adds up in the CTAs' order.
-constexpr int kNormGradMaxThreads = 256;
+//
+// Rows reach a lane through shared memory: it copies its own pieces there asynchronously, rows ahead of the one it works on, and reads
+// them back itself, so nothing but its own copies has to be waited for.  In registers there is room for one row ahead beside 64 column
+// sums, and 8 warps with one row each on its way are too few bytes for the memory's latency (59 us where this takes
+// 48, 30,001 x 784 float32).
+constexpr int kNormGradMaxThreads = 256;   // a row's group
+constexpr int kNormGradRegs = 168;         // so that 12 warps fit a processor
+template <int NV> constexpr int norm_grad_ahead() { return NV <= 4 ? 3 : 2; }      // rows in shared memory: 16 KB a warp at most
 template <typename T, typename P, int NV, bool ALIGNED>
-__global__ void __launch_bounds__(kNormGradMaxThreads)
+__global__ void __maxnreg__(kNormGradRegs)
 norm_grad_rows_kernel(const T* dy, long long dys, const T* x, long long xs, const float* mean, const float* rstd, int rows, int d,
                       float inv_d, const P* w, T* dx, long long dxs, float* part) {
-  constexpr int V = Piece<T>::V, H = V / 2;
+  constexpr int V = Piece<T>::V, H = V / 2, S = norm_grad_ahead<NV>();
   __shared__ float2 red[2][8];      // used in turn: one half may still be read by slower warps
+  extern __shared__ uint4 ring[];   // [warp][S][x, dy][NV][lane]; in the end the CTA's sums
   const int group = blockDim.x, per_cta = blockDim.y, which = threadIdx.y, in_group = threadIdx.x, lane = threadIdx.x & 31;
   const int warps = group / 32;
   const int first = in_group / 32 * (32 * NV) + lane;      // as in norm_rows_kernel
   const int have = min(NV, max(0, ((d + V - 1) / V - first + 31) / 32));
   float2 aw[NV][H], ab[NV][H];
+#pragma unroll
+  for (int p = 0; p < NV; ++p)
+#pragma unroll
+    for (int e = 0; e < H; ++e) aw[p][e] = ab[p][e] = both(0.f);
+  const int step = gridDim.x * per_cta;
+  int t = blockIdx.x * per_cta + which, turn = 0;
   struct Row {
     Piece<T> x[NV], g[NV];
     float mu, r;
   };
-  Row one, two;      // the next row is on its way into one while the other one's sums are formed
+  uint4* slots = ring + (which * warps + in_group / 32) * (S * 2 * NV * 32) + lane;
+  const auto copy = [&](int row, int slot) {      // ALIGNED: starts the copies of a row
+    if (row < rows) {
+      const uint4* xq = reinterpret_cast<const uint4*>(x + (long long)row * xs) + first;
+      const uint4* gq = reinterpret_cast<const uint4*>(dy + (long long)row * dys) + first;
+      uint4* to = slots + slot * (2 * NV * 32);
 #pragma unroll
-  for (int p = 0; p < NV; ++p) {
-    one.x[p].q = one.g[p].q = two.x[p].q = two.g[p].q = make_uint4(0u, 0u, 0u, 0u);
-#pragma unroll
-    for (int e = 0; e < H; ++e) aw[p][e] = ab[p][e] = both(0.f);
-  }
-  const int step = gridDim.x * per_cta;
-  int t = blockIdx.x * per_cta + which, turn = 0;
-  const auto load = [&](int row, Row& to) {
+      for (int p = 0; p < NV; ++p)
+        if (p < have) {
+          copy_async(to + p * 32, xq + p * 32);
+          copy_async(to + (NV + p) * 32, gq + p * 32);
+        }
+    }
+    copies_commit();
+  };
+  const auto load = [&](int row, Row& to) {       // not ALIGNED: the row itself
     if (row >= rows) return;
     load_pieces<T, NV, ALIGNED>(x + (long long)row * xs, first, have, d, to.x);
     load_pieces<T, NV, ALIGNED>(dy + (long long)row * dys, first, have, d, to.g);
-    to.mu = mean[row];
-    to.r = rstd[row];
   };
-  const auto grad = [&](const Row& row) {
+  const auto grad = [&](const Row& row, int slot) {
     const float r = row.r;
     const float2 rr = both(r), off = both(-row.mu * r);      // xh = x r - mu r: this rounding is no larger than the stored mean's
     float2 xh[NV][H], g[NV][H];
@@ -248,6 +266,7 @@ norm_grad_rows_kernel(const T* dy, long long dys, const T* x, long long xs, cons
     };
     if (w) sums(std::integral_constant<bool, true>());
     else sums(std::integral_constant<bool, false>());
+    if (ALIGNED) copy(t + S * step, slot);        // the row's values have been used: its place is free
     float s1 = warp_sum_f(a2.x + a2.y), s2 = warp_sum_f(b2.x + b2.y);
     if (warps > 1) {
       float2* mine = red[turn] + which * warps;
@@ -273,16 +292,46 @@ norm_grad_rows_kernel(const T* dy, long long dys, const T* x, long long xs, cons
     t += step;
     turn ^= 1;
   };
-  load(t, one);
-  while (t < rows) {
-    load(t + step, two);
-    grad(one);
-    if (t >= rows) break;
-    load(t + step, one);
-    grad(two);
+  float nmu = 0.f, nr = 0.f;
+  const auto statistics = [&](int row) {
+    if (row < rows) {
+      nmu = mean[row];
+      nr = rstd[row];
+    }
+  };
+  statistics(t);
+  if (ALIGNED) {
+    for (int i = 0; i < S * 2; ++i)
+      for (int p = have; p < NV; ++p) slots[(i * NV + p) * 32] = make_uint4(0u, 0u, 0u, 0u);     // pieces behind the row stay zero
+    for (int i = 0; i < S; ++i) copy(t + i * step, i);
+    int slot = 0;
+    while (t < rows) {
+      Row row;
+      row.mu = nmu;
+      row.r = nr;
+      copies_wait<S - 1>();
+#pragma unroll
+      for (int p = 0; p < NV; ++p) {
+        row.x[p].q = slots[(slot * 2 * NV + p) * 32];
+        row.g[p].q = slots[(slot * 2 * NV + NV + p) * 32];
+      }
+      statistics(t + step);
+      grad(row, slot);
+      slot = slot + 1 == S ? 0 : slot + 1;
+    }
+    copies_wait<0>();
+  } else {
+    Row row;
+    while (t < rows) {
+      load(t, row);
+      row.mu = nmu;
+      row.r = nr;
+      statistics(t + step);
+      grad(row, 0);
+    }
   }
   if (!part) return;
-  extern __shared__ float joined[];     // dw then db of the CTA, d each
+  float* joined = reinterpret_cast<float*>(ring);     // dw then db of the CTA, d each
   float* pw = part + (size_t)blockIdx.x * 2 * d;
   float* cols = per_cta > 1 ? joined : pw;
   for (int grp = 0; grp < per_cta; ++grp) {
@@ -304,6 +353,10 @@ norm_grad_rows_kernel(const T* dy, long long dys, const T* x, long long xs, cons
   if (per_cta > 1)
     for (int c = which * group + in_group; c < 2 * d; c += group * per_cta) pw[c] = cols[c];
 }
+
+// Shared memory of that kernel: the rows on their way.  (The sums of the groups that share a CTA, 2 d floats, take less.)
+template <typename T, int NV>
+constexpr size_t norm_grad_smem(int threads) { return (size_t)threads * (norm_grad_ahead<NV>() * 2 * NV * sizeof(uint4)); }
 
 // Rows wider than the registers take: one CTA per row, the row read again (from L2) for each of its sums.
 template <typename T, typename P>
@@ -388,7 +441,7 @@ norm_grad_sum_kernel(const float* part, int parts, int d, float* dw, float* db) 
 
 // CTAs of a walk: as many as run at once (per processor, from the kernel's registers).  Of the gradient's, each leaves a partial sum; their
 // number must not depend on more than the sizes and the element size, which is all that the workspace is asked for.
-constexpr int kNormGradThreadsPerSm = 256;
+constexpr int kNormGradThreadsPerSm = 384;
 inline NormShape norm_grad_shape(int d, int size) { return norm_shape(d, size, kNormGradMaxThreads); }
 inline int norm_grid(size_t rows, const NormShape& s, int sms, int threads_per_sm) {
   if (!s.group) return (int)std::min<size_t>(rows, (size_t)sms * 4);
@@ -434,9 +487,10 @@ template <typename T, typename P, bool ALIGNED>
 int norm_grad_launch(const NormShape& s, int grid, const T* dy, long long dys, const T* x, long long xs, const float* mean,
                      const float* rstd, int rows, int d, const P* w, T* dx, long long dxs, float* part, cudaStream_t stream) {
   return with_pieces<T>(s.nv, [&](auto nv) -> int {
-    // several groups a CTA: at most 2048 columns, 16 KB
-    const size_t smem = part && s.per_cta > 1 ? (size_t)2 * d * sizeof(float) : 0;
-    norm_grad_rows_kernel<T, P, nv(), ALIGNED><<<grid, dim3(s.group, s.per_cta), smem, stream>>>(
+    const auto fn = norm_grad_rows_kernel<T, P, nv(), ALIGNED>;
+    const size_t smem = norm_grad_smem<T, nv()>(s.threads());
+    KM_CUDA(allow_smem(fn, smem));
+    fn<<<grid, dim3(s.group, s.per_cta), smem, stream>>>(
         dy, dys, x, xs, mean, rstd, rows, d, 1.f / (float)d, w, dx, dxs, part);
     KM_CUDA(cudaGetLastError());
     return KM_OK;

@@ -92,6 +92,14 @@ __device__ __forceinline__ Piece<T> pack(const float2 (&f)[Piece<T>::V / 2]) {
   return p;
 }
 
+// Asynchronous copies of 16 bytes to shared memory, past L1; a thread waits for its own, all but the `N` newest groups.
+__device__ __forceinline__ void copy_async(uint4* to, const uint4* from) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((unsigned int)__cvta_generic_to_shared(to)), "l"(from) : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
 // Bytes [shift, shift + 16) of the 32 bytes a, b.
 __device__ __forceinline__ uint4 shift_words(uint4 a, uint4 b, unsigned int shift) {
   unsigned int w0 = a.x, w1 = a.y, w2 = a.z, w3 = a.w, w4 = b.x, w5 = b.y, w6 = b.z, w7 = b.w;
