@@ -1,4 +1,4 @@
-// Rows sorted by cluster and back.
+// Places of rows sorted by cluster.
 // Entry i = t n + j says that row t goes to cluster ids[i] (outside [0, k): nowhere).  A stable counting sort gives every entry
 // its place: groups in the clusters' order, each beginning on a multiple of `align`, entries of a group in their own order.
 //   slot[i] = place of entry i (-1: none);  source[p] = entry at place p (-1: padding)
@@ -154,74 +154,6 @@ sort_place_kernel(const int* ids, long long stride, int n, long long entries, in
         if (place >= 0) source[place] = (int)i;
       }
     }
-}
-
-constexpr int kMoveThreads = 256;
-
-// rows[slot(t, j)] = x[t]; places without an entry become zero rows.
-template <typename T>
-__global__ void __launch_bounds__(kMoveThreads)
-dispatch_kernel(const T* x, long long xs, int rows, int d, int n, const int* slot, const int* source, int capacity, T* out,
-                long long os) {
-  if (blockIdx.x < rows) {
-    const int t = blockIdx.x;
-    for (int c = threadIdx.x; c < d; c += kMoveThreads) {
-      const T v = x[(long long)t * xs + c];
-      for (int j = 0; j < n; ++j) {
-        const int p = slot[(long long)t * n + j];
-        if (p >= 0 && p < capacity) out[(long long)p * os + c] = v;
-      }
-    }
-    return;
-  }
-  for (int p = blockIdx.x - rows; p < capacity; p += gridDim.x - rows)
-    if (source[p] < 0)
-      for (int c = threadIdx.x; c < d; c += kMoveThreads) out[(long long)p * os + c] = from_f<T>(0.f);
-}
-
-// y[t] = sum over j of weights[t, j] in[slot(t, j)] (all weights one without them)
-template <typename T>
-__global__ void __launch_bounds__(kMoveThreads)
-combine_kernel(const T* in, long long is, int capacity, int d, const int* slot, const float* weights, int n, T* y, long long ys) {
-  const int t = blockIdx.x;
-  for (int c = threadIdx.x; c < d; c += kMoveThreads) {
-    float s = 0.f;
-    for (int j = 0; j < n; ++j) {
-      const int p = slot[(long long)t * n + j];
-      if (p < 0 || p >= capacity) continue;
-      s = fmaf(weights ? weights[(long long)t * n + j] : 1.f, to_f(in[(long long)p * is + c]), s);
-    }
-    y[(long long)t * ys + c] = from_f<T>(s);
-  }
-}
-
-// din[slot(t, j)] = weights[t, j] dy[t], zero rows where there is no entry; dweights[t, j] = <dy[t], in[slot(t, j)]>
-template <typename T>
-__global__ void __launch_bounds__(kMoveThreads)
-combine_grad_kernel(const T* dy, long long dys, const T* in, long long is, int capacity, int d, const int* slot, const int* source,
-                    const float* weights, int rows, int n, T* din, long long dis, float* dweights) {
-  __shared__ float red[32];
-  if (blockIdx.x < rows) {
-    const int t = blockIdx.x;
-    for (int j = 0; j < n; ++j) {
-      const int p = slot[(long long)t * n + j];
-      float s = 0.f;
-      if (p >= 0 && p < capacity) {
-        const float w = weights[(long long)t * n + j];
-        for (int c = threadIdx.x; c < d; c += kMoveThreads) {
-          const float g = to_f(dy[(long long)t * dys + c]);
-          s = fmaf(g, to_f(in[(long long)p * is + c]), s);
-          din[(long long)p * dis + c] = from_f<T>(w * g);
-        }
-      }
-      s = cta_sum(s, red);
-      if (threadIdx.x == 0) dweights[(long long)t * n + j] = s;
-    }
-    return;
-  }
-  for (int p = blockIdx.x - rows; p < capacity; p += gridDim.x - rows)
-    if (source[p] < 0)
-      for (int c = threadIdx.x; c < d; c += kMoveThreads) din[(long long)p * dis + c] = from_f<T>(0.f);
 }
 
 }  // namespace rows

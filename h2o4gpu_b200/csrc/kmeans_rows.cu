@@ -1,6 +1,7 @@
 // C entry points of the row operators (section 5 of include/h2o4gpu_kmeans.h): layer norm, routing to the nearest clusters,
 // rows sorted by cluster and back.  They work on device memory of the current device, enqueue on the caller's stream, never
 // allocate and never wait.
+#include "km_rows_move.cuh"
 #include "km_rows_norm.cuh"
 #include "km_rows_route.cuh"
 #include "km_rows_sort.cuh"
@@ -239,7 +240,10 @@ int check_move(const char* name, int dtype, size_t rows, int n, size_t cols, siz
   return KM_OK;
 }
 // CTAs that fill the places without an entry
-unsigned pad_ctas(size_t capacity, int sms) { return (unsigned)std::min<size_t>(capacity, (size_t)sms * 4); }
+unsigned pad_ctas(size_t capacity, int sms) {
+  return (unsigned)std::min<size_t>((capacity + kMoveThreads - 1) / kMoveThreads, (size_t)sms * 4);
+}
+int move_pieces(size_t cols, int size) { return (int)((cols * size + 15) / 16); }
 
 int dispatch(int dtype, const void* x, long long xs, size_t rows, size_t cols, int n, const int32_t* slot, const int32_t* source,
              size_t capacity, void* out, long long os, cudaStream_t stream) {
@@ -251,9 +255,13 @@ int dispatch(int dtype, const void* x, long long xs, size_t rows, size_t cols, i
     KM_FAIL(KM_EINVAL, "kmeans_dispatch: bad argument");
   int sms = 0;
   KM_TRY(sm_count(&sms));
+  const bool al = rows_aligned(x, xs, rows, cols, size) && rows_aligned(out, os, capacity, cols, size);
+  const long long blocks = rows ? move_blocks(rows, move_pieces(cols, size), al) : 0, grid = blocks + pad_ctas(capacity, sms);
+  if (grid > 0x7fffffffLL) KM_FAIL(KM_EINVAL, "kmeans_dispatch: too many rows for one launch");
   KM_ROWS_DTYPE(dtype, T,
-      dispatch_kernel<T><<<(unsigned)rows + pad_ctas(capacity, sms), kMoveThreads, 0, stream>>>(
-          static_cast<const T*>(x), xs, (int)rows, (int)cols, n, slot, source, (int)capacity, static_cast<T*>(out), os));
+      const auto fn = al ? dispatch_kernel<T, true> : dispatch_kernel<T, false>;
+      fn<<<(unsigned)grid, kMoveThreads, 0, stream>>>(static_cast<const T*>(x), xs, (int)rows, (int)cols, n, slot, source, (int)capacity,
+                                                      static_cast<T*>(out), os, blocks));
   KM_CUDA(cudaGetLastError());
   return KM_OK;
 }
@@ -266,9 +274,13 @@ int combine(int dtype, const void* in, long long is, size_t capacity, size_t col
   if ((capacity && !block_ok(in, is, capacity, cols, size, false)) || !slot || !aligned(slot, 4) || !aligned(weights, 4) ||
       !block_ok(y, ys, rows, cols, size, true))
     KM_FAIL(KM_EINVAL, "kmeans_combine: bad argument");
+  const bool al = rows_aligned(in, is, capacity, cols, size) && rows_aligned(y, ys, rows, cols, size);
+  const long long grid = move_blocks(rows, move_pieces(cols, size), al);
+  if (grid > 0x7fffffffLL) KM_FAIL(KM_EINVAL, "kmeans_combine: too many rows for one launch");
   KM_ROWS_DTYPE(dtype, T,
-      combine_kernel<T><<<(unsigned)rows, kMoveThreads, 0, stream>>>(static_cast<const T*>(in), is, (int)capacity, (int)cols, slot,
-                                                                      weights, n, static_cast<T*>(y), ys));
+      const auto fn = al ? combine_kernel<T, true> : combine_kernel<T, false>;
+      fn<<<(unsigned)grid, kMoveThreads, 0, stream>>>(static_cast<const T*>(in), is, (int)capacity, (int)cols, slot, weights, (int)rows,
+                                                      n, static_cast<T*>(y), ys));
   KM_CUDA(cudaGetLastError());
   return KM_OK;
 }
@@ -286,8 +298,12 @@ int combine_grad(int dtype, const void* dy, long long dys, const void* in, long 
     KM_FAIL(KM_EINVAL, "kmeans_combine_grad: bad argument");
   int sms = 0;
   KM_TRY(sm_count(&sms));
+  const bool al = rows_aligned(dy, dys, rows, cols, size) && rows_aligned(in, is, capacity, cols, size) &&
+                  rows_aligned(din, dis, capacity, cols, size);
+  const int threads = std::min(kMoveThreads, (move_pieces(cols, size) + 31) / 32 * 32);
   KM_ROWS_DTYPE(dtype, T,
-      combine_grad_kernel<T><<<(unsigned)rows + pad_ctas(capacity, sms), kMoveThreads, 0, stream>>>(
+      const auto fn = al ? combine_grad_kernel<T, true> : combine_grad_kernel<T, false>;
+      fn<<<(unsigned)rows + pad_ctas(capacity, sms), threads, 0, stream>>>(
           static_cast<const T*>(dy), dys, static_cast<const T*>(in), is, (int)capacity, (int)cols, slot, source, weights, (int)rows,
           n, static_cast<T*>(din), dis, dweights));
   KM_CUDA(cudaGetLastError());
