@@ -11,35 +11,24 @@ namespace rows {
 
 constexpr int kMoveThreads = 256;
 
-// Work is cut into pieces of 16 bytes.  Aligned rows: piece i of all rows together goes to thread i, so narrow rows fill warps too.  Others:
-// a warp takes 32 consecutive pieces of one row (the lanes pass each other what lies across two words).
+// Work is cut into words of 16 bytes of the rows that are written: word i of a row holds its columns from i V - before_row on.  Those of
+// the rows that are read may lie across two words there (load_window).  Words of all rows together go to consecutive threads, so that
+// narrow rows fill warps too.
 struct MoveItem {
-  int row, piece;
-  bool valid;
+  int row, word;
 };
-template <bool ALIGNED>
-__device__ __forceinline__ MoveItem move_item(long long block, int rows, int pieces) {
-  MoveItem m;
-  const long long thread = block * kMoveThreads + threadIdx.x;
-  if (ALIGNED) {
-    // (32-bit division while the numbers allow it)
-    const long long r = thread <= 0xffffffffLL ? (long long)((unsigned int)thread / (unsigned int)pieces) : thread / pieces;
-    m.row = (int)r;
-    m.piece = (int)(thread - r * pieces);
-    m.valid = r < rows;
-  } else {
-    const int per_row = (pieces + 31) / 32;
-    const long long warp = thread / 32, r = warp / per_row;
-    m.row = (int)r;
-    m.piece = (int)(warp - r * per_row) * 32 + (threadIdx.x & 31);
-    m.valid = r < rows;      // a whole warp
-  }
-  return m;
+__device__ __forceinline__ MoveItem move_item(int words) {
+  const long long thread = (long long)blockIdx.x * kMoveThreads + threadIdx.x;
+  // (32-bit division while the numbers allow it)
+  const long long r = thread <= 0xffffffffLL ? (long long)((unsigned int)thread / (unsigned int)words) : thread / words;
+  return {(int)min(r, 0x7fffffffLL), (int)(thread - r * words)};
 }
-inline long long move_blocks(size_t rows, int pieces, bool al) {
-  const long long threads = al ? (long long)rows * pieces : (long long)rows * ((pieces + 31) / 32) * 32;
-  return (threads + kMoveThreads - 1) / kMoveThreads;
+// Words that a row can lie across.
+inline int move_words(size_t cols, int size, bool al) {
+  const size_t v = 16 / size;
+  return (int)(al ? cols / v : (cols + 2 * v - 2) / v);
 }
+inline long long move_blocks(size_t rows, int words) { return ((long long)rows * words + kMoveThreads - 1) / kMoveThreads; }
 
 template <typename T>
 __device__ __forceinline__ Piece<T> zero_piece() {
@@ -47,46 +36,69 @@ __device__ __forceinline__ Piece<T> zero_piece() {
   p.q = make_uint4(0u, 0u, 0u, 0u);
   return p;
 }
+// The V elements at column c of a row.
+template <typename T, bool ALIGNED>
+__device__ __forceinline__ Piece<T> load_at(const T* row, int c, const Span<T>& in) {
+  if (!ALIGNED) return load_window(row + c, in);
+  Piece<T> p;
+  p.q = *reinterpret_cast<const uint4*>(row + c);
+  return p;
+}
 
 // Zero rows at the places without an entry: warp by warp over the places.
-template <typename T, bool ALIGNED>
+template <typename T>
 __device__ __forceinline__ void zero_unused(T* out, long long os, int d, const int* source, int capacity, long long block,
                                             long long blocks) {
-  const int lane = threadIdx.x & 31, pieces = (d + Piece<T>::V - 1) / Piece<T>::V;
-  for (long long p0 = (block * blockDim.x + threadIdx.x) / 32 * 32; p0 < capacity; p0 += blocks * blockDim.x) {
+  constexpr int V = Piece<T>::V;
+  const int tid = threadIdx.x + threadIdx.y * blockDim.x, threads = blockDim.x * blockDim.y, lane = tid & 31;
+  for (long long p0 = (block * threads + tid) / 32 * 32; p0 < capacity; p0 += blocks * threads) {
     const bool mine = p0 + lane < capacity && source[p0 + lane] < 0;
     for (unsigned int left = __ballot_sync(0xffffffffu, mine); left; left &= left - 1) {
       T* row = out + (p0 + __ffs(left) - 1) * os;
-      for (int i = lane; i < (pieces + 31) / 32 * 32; i += 32) store_piece<T, ALIGNED>(row, i, d, zero_piece<T>());
+      for (int c = lane * V - before_row(row); c < d; c += 32 * V) store_word(row, c, d, zero_piece<T>());
     }
   }
 }
 
 template <typename T, bool ALIGNED>
 __global__ void __launch_bounds__(kMoveThreads)
-dispatch_kernel(const T* x, long long xs, int rows, int d, int n, const int* slot, const int* source, int capacity, T* out,
-                long long os, long long blocks) {
+dispatch_kernel(const T* x, long long xs, Span<T> xin, int rows, int d, int words, int n, const int* slot, const int* source,
+                int capacity, T* out, long long os, long long blocks) {
+  constexpr int V = Piece<T>::V;
   if (blockIdx.x >= blocks) {
-    zero_unused<T, ALIGNED>(out, os, d, source, capacity, blockIdx.x - blocks, gridDim.x - blocks);
+    zero_unused(out, os, d, source, capacity, blockIdx.x - blocks, gridDim.x - blocks);
     return;
   }
-  const MoveItem m = move_item<ALIGNED>(blockIdx.x, rows, (d + Piece<T>::V - 1) / Piece<T>::V);
-  if (!m.valid) return;
-  const Piece<T> v = load_piece<T, ALIGNED>(x + m.row * xs, m.piece, d);
+  const MoveItem m = move_item(words);
+  if (m.row >= rows) return;
+  const T* row = x + m.row * xs;
   const int* sl = slot + (long long)m.row * n;
+  Piece<T> v;
+  if (ALIGNED) v = load_at<T, true>(row, m.word * V, xin);
   for (int j = 0; j < n; ++j) {
     const int p = sl[j];
-    if (p >= 0 && p < capacity) store_piece<T, ALIGNED>(out + p * os, m.piece, d, v);
+    if (p < 0 || p >= capacity) continue;
+    T* to = out + p * os;
+    if (ALIGNED) {
+      *reinterpret_cast<uint4*>(to + m.word * V) = v.q;
+    } else {
+      const int c = m.word * V - before_row(to);
+      if (c < d) store_word(to, c, d, load_at<T, false>(row, c, xin));
+    }
   }
 }
 
-template <typename T, bool ALIGNED>
+// AT_ONCE entries are on their way together.
+template <typename T, bool ALIGNED, int AT_ONCE>
 __global__ void __launch_bounds__(kMoveThreads)
-combine_kernel(const T* in, long long is, int capacity, int d, const int* slot, const float* weights, int rows, int n, T* y,
-               long long ys) {
-  constexpr int H = Piece<T>::V / 2, AT_ONCE = 4;
-  const MoveItem m = move_item<ALIGNED>(blockIdx.x, rows, (d + Piece<T>::V - 1) / Piece<T>::V);
-  if (!m.valid) return;
+combine_kernel(const T* in, long long is, Span<T> iin, int capacity, int d, int words, const int* slot, const float* weights, int rows,
+               int n, T* y, long long ys) {
+  constexpr int V = Piece<T>::V, H = V / 2;
+  const MoveItem m = move_item(words);
+  if (m.row >= rows) return;
+  T* to = y + m.row * ys;
+  const int c = m.word * V - (ALIGNED ? 0 : before_row(to));
+  if (c >= d) return;
   const int* sl = slot + (long long)m.row * n;
   const float* w = weights ? weights + (long long)m.row * n : nullptr;
   float2 sum[H];
@@ -100,8 +112,9 @@ combine_kernel(const T* in, long long is, int capacity, int d, const int* slot, 
     for (int u = 0; u < AT_ONCE; ++u) {
       const int p = j0 + u < n ? sl[j0 + u] : -1;
       there[u] = p >= 0 && p < capacity;
-      f[u] = there[u] && w ? w[j0 + u] : 1.f;
-      v[u] = there[u] ? load_piece<T, ALIGNED>(in + p * is, m.piece, d) : zero_piece<T>();
+      if (!there[u]) continue;
+      f[u] = w ? w[j0 + u] : 1.f;
+      v[u] = load_at<T, ALIGNED>(in + p * is, c, iin);
     }
 #pragma unroll
     for (int u = 0; u < AT_ONCE; ++u) {
@@ -112,54 +125,109 @@ combine_kernel(const T* in, long long is, int capacity, int d, const int* slot, 
       for (int e = 0; e < H; ++e) sum[e] = fma2(both(f[u]), g[e], sum[e]);
     }
   }
-  store_piece<T, ALIGNED>(y + m.row * ys, m.piece, d, pack<T>(sum));
+  const Piece<T> o = pack<T>(sum);
+  if (ALIGNED) *reinterpret_cast<uint4*>(to + c) = o.q;
+  else store_word(to, c, d, o);
 }
 
-// One CTA per row, its threads over the row's pieces; the dot products of up to 32 entries are joined over the warps at once.
-template <typename T, bool ALIGNED>
+// blockDim.x threads (whole warps) take a row, blockDim.y rows share a CTA; the dot products are joined over a row's warps, 32 entries at
+// a time.
+template <typename T, bool ALIGNED, int AT_ONCE>
 __global__ void __launch_bounds__(kMoveThreads)
-combine_grad_kernel(const T* dy, long long dys, const T* in, long long is, int capacity, int d, const int* slot, const int* source,
-                    const float* weights, int rows, int n, T* din, long long dis, float* dweights) {
-  constexpr int H = Piece<T>::V / 2;
-  __shared__ float red[32][kMoveThreads / 32 + 1];
-  if ((int)blockIdx.x >= rows) {
-    zero_unused<T, ALIGNED>(din, dis, d, source, capacity, blockIdx.x - rows, gridDim.x - rows);
+combine_grad_kernel(const T* dy, long long dys, Span<T> gin, const T* in, long long is, Span<T> iin, int capacity, int d, int words,
+                    const int* slot, const int* source, const float* weights, int rows, int n, T* din, long long dis, float* dweights,
+                    int blocks) {
+  constexpr int V = Piece<T>::V, H = V / 2;
+  __shared__ float red[kMoveThreads / 32][32];
+  if ((int)blockIdx.x >= blocks) {
+    zero_unused(din, dis, d, source, capacity, blockIdx.x - blocks, gridDim.x - blocks);
     return;
   }
-  const int t = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x / 32, warps = blockDim.x / 32;
-  const int pieces = ((d + Piece<T>::V - 1) / Piece<T>::V + 31) / 32 * 32;
+  const int t = blockIdx.x * blockDim.y + threadIdx.y, lane = threadIdx.x & 31, warps = blockDim.x / 32;
+  const bool valid = t < rows;
+  const T* gr = dy + t * dys;
   for (int j0 = 0; j0 < n; j0 += 32) {
     const int nj = min(32, n - j0);
-    for (int j = 0; j < nj; ++j) {
-      const long long at = (long long)t * n + j0 + j;
-      const int p = slot[at];
-      float dot = 0.f;
-      if (p >= 0 && p < capacity) {
-        const float2 w = both(weights[at]);
-        float2 s = both(0.f);
-        for (int i = threadIdx.x; i < pieces; i += blockDim.x) {
-          float2 g[H], v[H];
-          unpack(load_piece<T, ALIGNED>(dy + t * dys, i, d), g);
-          unpack(load_piece<T, ALIGNED>(in + p * is, i, d), v);
+    float mine = 0.f;       // lane j: this warp's part of entry j
+    for (int u0 = 0; u0 < nj; u0 += AT_ONCE) {
+      int p[AT_ONCE];
+      float w[AT_ONCE];
+      float2 dot[AT_ONCE];
+      const T* from[AT_ONCE];
+      T* to[AT_ONCE];
+#pragma unroll
+      for (int u = 0; u < AT_ONCE; ++u) {
+        const long long at = (long long)t * n + j0 + u0 + u;
+        p[u] = valid && u0 + u < nj ? slot[at] : -1;
+        if (p[u] >= capacity) p[u] = -1;
+        w[u] = p[u] >= 0 ? weights[at] : 0.f;
+        from[u] = in + (long long)max(p[u], 0) * is;
+        to[u] = din + (long long)max(p[u], 0) * dis;
+        dot[u] = both(0.f);
+      }
+      for (int i = threadIdx.x; i < words; i += blockDim.x) {
+        Piece<T> g, v[AT_ONCE], gu[AT_ONCE];
+        if (ALIGNED) g = load_at<T, true>(gr, valid ? i * V : 0, gin);
+#pragma unroll
+        for (int u = 0; u < AT_ONCE; ++u) {
+          if (p[u] < 0) continue;
+          const int c = i * V - (ALIGNED ? 0 : before_row(to[u]));
+          if (!ALIGNED && c >= d) {
+            gu[u] = v[u] = zero_piece<T>();
+            continue;
+          }
+          v[u] = load_at<T, ALIGNED>(from[u], c, iin);
+          if (!ALIGNED) {
+            gu[u] = load_at<T, false>(gr, c, gin);
+            clip_piece(gu[u], c, d);
+            clip_piece(v[u], c, d);
+          }
+        }
+#pragma unroll
+        for (int u = 0; u < AT_ONCE; ++u) {
+          if (p[u] < 0) continue;
+          float2 a[H], b[H];
+          unpack(ALIGNED ? g : gu[u], a);
+          unpack(v[u], b);
 #pragma unroll
           for (int e = 0; e < H; ++e) {
-            s = fma2(g[e], v[e], s);
-            g[e] = mul2(g[e], w);
+            dot[u] = fma2(a[e], b[e], dot[u]);
+            a[e] = mul2(a[e], both(w[u]));
           }
-          store_piece<T, ALIGNED>(din + p * dis, i, d, pack<T>(g));
+          const Piece<T> o = pack<T>(a);
+          if (ALIGNED) {
+            *reinterpret_cast<uint4*>(to[u] + i * V) = o.q;
+          } else {
+            const int c = i * V - before_row(to[u]);
+            if (c < d) store_word(to[u], c, d, o);
+          }
         }
-        dot = warp_sum_f(s.x + s.y);
       }
-      if (lane == 0) red[j][warp] = dot;
+#pragma unroll
+      for (int u = 0; u < AT_ONCE; ++u) {
+        const float s = warp_sum_f(dot[u].x + dot[u].y);
+        if (lane == u0 + u) mine = s;
+      }
     }
-    __syncthreads();
-    if ((int)threadIdx.x < nj) {
-      float s = 0.f;
-      for (int i = 0; i < warps; ++i) s += red[threadIdx.x][i];
-      dweights[(long long)t * n + j0 + threadIdx.x] = s;
+    if (warps > 1) {
+      float* row = red[threadIdx.y * warps];
+      red[threadIdx.y * warps + threadIdx.x / 32][lane] = mine;
+      __syncthreads();
+      mine = 0.f;
+      if (threadIdx.x < 32)
+        for (int i = 0; i < warps; ++i) mine += row[i * 32 + lane];
+      __syncthreads();
     }
-    __syncthreads();
+    if (valid && threadIdx.x < 32 && lane < nj) dweights[(long long)t * n + j0 + lane] = mine;
   }
+}
+
+// Warps for a row: one (its lanes keep many loads on their way, nothing is joined) while there are rows for all warps that fit the device
+// (64 a processor), more for fewer rows.
+inline int combine_grad_warps(size_t rows, int words, int sms) {
+  int w = 1;
+  while (w < kMoveThreads / 32 && (words + 31) / 32 > w && rows * w < (size_t)sms * 64) w *= 2;
+  return w;
 }
 
 }  // namespace rows

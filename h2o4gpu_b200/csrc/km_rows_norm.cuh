@@ -40,14 +40,14 @@ __device__ __forceinline__ void load_params(const P* w, int i, int d, bool insid
 // Pieces of a row that a lane holds: `have` of them lie in the row, the others are never loaded and stay zero (a load that
 // fills in zeros, addresses that are formed for every piece and row cost more instructions than the sums).
 template <typename T, int NV, bool ALIGNED>
-__device__ __forceinline__ void load_pieces(const T* row, int first, int have, int d, Piece<T> (&p)[NV]) {
+__device__ __forceinline__ void load_pieces(const T* row, int first, int have, int d, const Span<T>& in, Piece<T> (&p)[NV]) {
   const uint4* q = reinterpret_cast<const uint4*>(row) + first;
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     if (ALIGNED) {
       if (i < have) p[i].q = q[i * 32];
     } else {
-      p[i] = load_piece<T, false>(row, first + i * 32, d);
+      p[i] = load_piece<T, false>(row, first + i * 32, d, in);
     }
   }
 }
@@ -82,7 +82,7 @@ __device__ __forceinline__ void group_sync() {
 constexpr int kNormMaxThreads = 512;       // a row's group
 template <typename T, typename P, int NV, bool ALIGNED>
 __global__ void __launch_bounds__(kNormMaxThreads)
-norm_rows_kernel(const T* x, long long xs, int rows, int d, float inv_d, const P* w, const P* b, float eps, T* y, long long ys,
+norm_rows_kernel(const T* x, long long xs, Span<T> xin, int rows, int d, float inv_d, const P* w, const P* b, float eps, T* y, long long ys,
                  float* mean, float* rstd) {
   constexpr int V = Piece<T>::V, H = V / 2;
   __shared__ float2 red[2][16];      // used in turn: one half may still be read by slower warps
@@ -100,7 +100,7 @@ norm_rows_kernel(const T* x, long long xs, int rows, int d, float inv_d, const P
 #pragma unroll
   for (int p = 0; p < NV; ++p) one[p].q = two[p].q = make_uint4(0u, 0u, 0u, 0u);
   const auto load = [&](int row, Piece<T>(&p)[NV]) {
-    if (row < rows) load_pieces<T, NV, ALIGNED>(x + (long long)row * xs, first, have, d, p);
+    if (row < rows) load_pieces<T, NV, ALIGNED>(x + (long long)row * xs, first, have, d, xin, p);
   };
   const auto norm = [&](const Piece<T>(&raw)[NV]) {
     float2 v[NV][H];
@@ -198,7 +198,7 @@ constexpr int kNormGradRegs = 168;         // so that 12 warps fit a processor
 template <int NV> constexpr int norm_grad_ahead() { return NV <= 4 ? 3 : 2; }      // rows in shared memory: 16 KB a warp at most
 template <typename T, typename P, int NV, bool ALIGNED>
 __global__ void __maxnreg__(kNormGradRegs)
-norm_grad_rows_kernel(const T* dy, long long dys, const T* x, long long xs, const float* mean, const float* rstd, int rows, int d,
+norm_grad_rows_kernel(const T* dy, long long dys, Span<T> gin, const T* x, long long xs, Span<T> xin, const float* mean, const float* rstd, int rows, int d,
                       float inv_d, const P* w, T* dx, long long dxs, float* part) {
   constexpr int V = Piece<T>::V, H = V / 2, S = norm_grad_ahead<NV>();
   __shared__ float2 red[2][8];      // used in turn: one half may still be read by slower warps
@@ -235,8 +235,8 @@ norm_grad_rows_kernel(const T* dy, long long dys, const T* x, long long xs, cons
   };
   const auto load = [&](int row, Row& to) {       // not ALIGNED: the row itself
     if (row >= rows) return;
-    load_pieces<T, NV, ALIGNED>(x + (long long)row * xs, first, have, d, to.x);
-    load_pieces<T, NV, ALIGNED>(dy + (long long)row * dys, first, have, d, to.g);
+    load_pieces<T, NV, ALIGNED>(x + (long long)row * xs, first, have, d, xin, to.x);
+    load_pieces<T, NV, ALIGNED>(dy + (long long)row * dys, first, have, d, gin, to.g);
   };
   const auto grad = [&](const Row& row, int slot) {
     const float r = row.r;
@@ -476,7 +476,7 @@ int norm_launch(const NormShape& s, int sms, const T* x, long long xs, int rows,
     int per_sm = 0;
     KM_TRY(resident.get(fn, s.threads(), &per_sm));
     const int grid = norm_grid(rows, s, sms, per_sm * s.threads());
-    fn<<<grid, dim3(s.group, s.per_cta), 0, stream>>>(x, xs, rows, d, 1.f / (float)d, w, b, eps, y,
+    fn<<<grid, dim3(s.group, s.per_cta), 0, stream>>>(x, xs, span_of<T>(x, xs, rows, d), rows, d, 1.f / (float)d, w, b, eps, y,
                                                                                         ys, mean, rstd);
     KM_CUDA(cudaGetLastError());
     return KM_OK;
@@ -491,7 +491,8 @@ int norm_grad_launch(const NormShape& s, int grid, const T* dy, long long dys, c
     const size_t smem = norm_grad_smem<T, nv()>(s.threads());
     KM_CUDA(allow_smem(fn, smem));
     fn<<<grid, dim3(s.group, s.per_cta), smem, stream>>>(
-        dy, dys, x, xs, mean, rstd, rows, d, 1.f / (float)d, w, dx, dxs, part);
+        dy, dys, span_of<T>(dy, dys, rows, d), x, xs, span_of<T>(x, xs, rows, d), mean, rstd, rows, d, 1.f / (float)d, w, dx, dxs,
+        part);
     KM_CUDA(cudaGetLastError());
     return KM_OK;
   });

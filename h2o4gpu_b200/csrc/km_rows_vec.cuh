@@ -1,8 +1,8 @@
 // Rows in 16-byte pieces, whatever their alignment.
 // Piece i of a row is its elements [i V, i V + V).  Where rows start on 16-byte boundaries a piece is one load or store.  Elsewhere a
 // piece lies across two aligned words of 16 bytes: a load takes both and shifts (the second is the next lane's first, so it comes from
-// L1), a store passes what does not fit its own word to the next lane.  Words that stick out of the row are taken apart element by
-// element: nothing outside the row is touched.
+// L1), a store passes what does not fit its own word to the next lane.  A word may hold elements beside the row, but never any outside the
+// block that the rows belong to (Span): there it is taken apart element by element.
 #pragma once
 
 #include "km_rows.cuh"
@@ -110,33 +110,82 @@ __device__ __forceinline__ uint4 shift_words(uint4 a, uint4 b, unsigned int shif
                     __funnelshift_r(w3, w4, bits));
 }
 
+// From the first element of a block's first row to behind the last one of its last row.
+template <typename T>
+struct Span {
+  const T* lo;
+  const T* hi;
+};
+template <typename T>
+inline Span<T> span_of(const void* p, long long stride, size_t rows, size_t cols) {
+  const T* lo = static_cast<const T*>(p);
+  return {lo, rows ? lo + (long long)(rows - 1) * stride + cols : lo};
+}
+
+// V elements from `from` on (any alignment); what lies outside the span is zero.
+template <typename T>
+__device__ __forceinline__ Piece<T> load_window(const T* from, const Span<T>& in) {
+  constexpr int V = Piece<T>::V;
+  Piece<T> p;
+  const unsigned int off = (unsigned int)(reinterpret_cast<uintptr_t>(from) & 15);
+  const T* word = from - off / sizeof(T);
+  if (word >= in.lo && word + (off ? 2 * V : V) <= in.hi) {
+    const uint4 a = *reinterpret_cast<const uint4*>(word);
+    p.q = off ? shift_words(a, *reinterpret_cast<const uint4*>(word + V), off) : a;
+    return p;
+  }
+  p.q = make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+  for (int e = 0; e < V; ++e)
+    if (from + e >= in.lo && from + e < in.hi) p.e[e] = from[e];
+  return p;
+}
+
+// The elements of a piece that starts at column c and lie outside [0, d) become zero.
+template <typename T>
+__device__ __forceinline__ void clip_piece(Piece<T>& p, int c, int d) {
+  constexpr int V = Piece<T>::V;
+  if (c >= 0 && c + V <= d) return;
+#pragma unroll
+  for (int e = 0; e < V; ++e)
+    if (c + e < 0 || c + e >= d) p.e[e] = from_f<T>(0.f);
+}
+
 // Piece i of the row at `row` with d elements; zeros behind the row's end.  ALIGNED: the row starts on a 16-byte boundary and is
 // whole pieces long.
 template <typename T, bool ALIGNED>
-__device__ __forceinline__ Piece<T> load_piece(const T* row, int i, int d) {
+__device__ __forceinline__ Piece<T> load_piece(const T* row, int i, int d, const Span<T>& in) {
   constexpr int V = Piece<T>::V;
   Piece<T> p;
   const int c = i * V;
   if (ALIGNED) {
     p.q = c < d ? *reinterpret_cast<const uint4*>(row + c) : make_uint4(0u, 0u, 0u, 0u);
     return p;
-  } else {
-    const unsigned int off = (unsigned int)(reinterpret_cast<uintptr_t>(row) & 15);
-    // first element of the two words, counted from the row's start, and one behind their last
-    const int first = c - (int)(off / sizeof(T)), behind = first + (off ? 2 : 1) * V;
-    if (first >= 0 && behind <= d) {
-      const uint4* word = reinterpret_cast<const uint4*>(row + first);
-      const uint4 a = word[0];
-      p.q = off ? shift_words(a, word[1], off) : a;
-      return p;
-    }
   }
-  p.q = make_uint4(0u, 0u, 0u, 0u);
-#pragma unroll
-  for (int e = 0; e < V; ++e)
-    if (c + e < d) p.e[e] = row[c + e];
+  if (c >= d) {
+    p.q = make_uint4(0u, 0u, 0u, 0u);
+    return p;
+  }
+  p = load_window(row + c, in);
+  clip_piece(p, c, d);
   return p;
 }
+
+// Stores the elements of `p` that lie in [0, d), the first at column c of the row; row + c is a 16-byte boundary.
+template <typename T>
+__device__ __forceinline__ void store_word(T* row, int c, int d, const Piece<T>& p) {
+  constexpr int V = Piece<T>::V;
+  if (c >= 0 && c + V <= d) {
+    *reinterpret_cast<uint4*>(row + c) = p.q;
+    return;
+  }
+#pragma unroll
+  for (int e = 0; e < V; ++e)
+    if (c + e >= 0 && c + e < d) row[c + e] = p.e[e];
+}
+// Elements of the row's first word that lie before the row.
+template <typename T>
+__device__ __forceinline__ int before_row(const T* row) { return (int)((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(T)); }
 
 // Stores piece i of the row.  Not ALIGNED: all 32 lanes call it with consecutive pieces (lane 0 the first); pieces behind
 // the row's end store nothing.

@@ -243,7 +243,6 @@ int check_move(const char* name, int dtype, size_t rows, int n, size_t cols, siz
 unsigned pad_ctas(size_t capacity, int sms) {
   return (unsigned)std::min<size_t>((capacity + kMoveThreads - 1) / kMoveThreads, (size_t)sms * 4);
 }
-int move_pieces(size_t cols, int size) { return (int)((cols * size + 15) / 16); }
 
 int dispatch(int dtype, const void* x, long long xs, size_t rows, size_t cols, int n, const int32_t* slot, const int32_t* source,
              size_t capacity, void* out, long long os, cudaStream_t stream) {
@@ -256,15 +255,24 @@ int dispatch(int dtype, const void* x, long long xs, size_t rows, size_t cols, i
   int sms = 0;
   KM_TRY(sm_count(&sms));
   const bool al = rows_aligned(x, xs, rows, cols, size) && rows_aligned(out, os, capacity, cols, size);
-  const long long blocks = rows ? move_blocks(rows, move_pieces(cols, size), al) : 0, grid = blocks + pad_ctas(capacity, sms);
+  const int words = move_words(cols, size, al);
+  const long long blocks = move_blocks(rows, words), grid = blocks + pad_ctas(capacity, sms);
   if (grid > 0x7fffffffLL) KM_FAIL(KM_EINVAL, "kmeans_dispatch: too many rows for one launch");
   KM_ROWS_DTYPE(dtype, T,
       const auto fn = al ? dispatch_kernel<T, true> : dispatch_kernel<T, false>;
-      fn<<<(unsigned)grid, kMoveThreads, 0, stream>>>(static_cast<const T*>(x), xs, (int)rows, (int)cols, n, slot, source, (int)capacity,
-                                                      static_cast<T*>(out), os, blocks));
+      fn<<<(unsigned)grid, kMoveThreads, 0, stream>>>(static_cast<const T*>(x), xs, span_of<T>(x, xs, rows, cols), (int)rows, (int)cols,
+                                                      words, n, slot, source, (int)capacity, static_cast<T*>(out), os, blocks));
   KM_CUDA(cudaGetLastError());
   return KM_OK;
 }
+
+// How many entries of a row are on their way together: no more than there are.
+#define KM_ROWS_AT_ONCE(n, U, ...)                                                         \
+  do {                                                                                     \
+    if ((n) == 1) { constexpr int U = 1; __VA_ARGS__; }                                    \
+    else if ((n) == 2) { constexpr int U = 2; __VA_ARGS__; }                               \
+    else { constexpr int U = 4; __VA_ARGS__; }                                             \
+  } while (0)
 
 int combine(int dtype, const void* in, long long is, size_t capacity, size_t cols, const int32_t* slot, const float* weights,
             size_t rows, int n, void* y, long long ys, cudaStream_t stream) {
@@ -275,12 +283,13 @@ int combine(int dtype, const void* in, long long is, size_t capacity, size_t col
       !block_ok(y, ys, rows, cols, size, true))
     KM_FAIL(KM_EINVAL, "kmeans_combine: bad argument");
   const bool al = rows_aligned(in, is, capacity, cols, size) && rows_aligned(y, ys, rows, cols, size);
-  const long long grid = move_blocks(rows, move_pieces(cols, size), al);
+  const int words = move_words(cols, size, al);
+  const long long grid = move_blocks(rows, words);
   if (grid > 0x7fffffffLL) KM_FAIL(KM_EINVAL, "kmeans_combine: too many rows for one launch");
-  KM_ROWS_DTYPE(dtype, T,
-      const auto fn = al ? combine_kernel<T, true> : combine_kernel<T, false>;
-      fn<<<(unsigned)grid, kMoveThreads, 0, stream>>>(static_cast<const T*>(in), is, (int)capacity, (int)cols, slot, weights, (int)rows,
-                                                      n, static_cast<T*>(y), ys));
+  KM_ROWS_DTYPE(dtype, T, KM_ROWS_AT_ONCE(n, U,
+      const auto fn = al ? combine_kernel<T, true, U> : combine_kernel<T, false, U>;
+      fn<<<(unsigned)grid, kMoveThreads, 0, stream>>>(static_cast<const T*>(in), is, span_of<T>(in, is, capacity, cols), (int)capacity,
+                                                      (int)cols, words, slot, weights, (int)rows, n, static_cast<T*>(y), ys)));
   KM_CUDA(cudaGetLastError());
   return KM_OK;
 }
@@ -300,12 +309,14 @@ int combine_grad(int dtype, const void* dy, long long dys, const void* in, long 
   KM_TRY(sm_count(&sms));
   const bool al = rows_aligned(dy, dys, rows, cols, size) && rows_aligned(in, is, capacity, cols, size) &&
                   rows_aligned(din, dis, capacity, cols, size);
-  const int threads = std::min(kMoveThreads, (move_pieces(cols, size) + 31) / 32 * 32);
-  KM_ROWS_DTYPE(dtype, T,
-      const auto fn = al ? combine_grad_kernel<T, true> : combine_grad_kernel<T, false>;
-      fn<<<(unsigned)rows + pad_ctas(capacity, sms), threads, 0, stream>>>(
-          static_cast<const T*>(dy), dys, static_cast<const T*>(in), is, (int)capacity, (int)cols, slot, source, weights, (int)rows,
-          n, static_cast<T*>(din), dis, dweights));
+  const int words = move_words(cols, size, al), warps = combine_grad_warps(rows, words, sms), per_cta = kMoveThreads / 32 / warps;
+  const int blocks = (int)((rows + per_cta - 1) / per_cta);
+  KM_ROWS_DTYPE(dtype, T, KM_ROWS_AT_ONCE(n, U,
+      const auto fn = al ? combine_grad_kernel<T, true, U> : combine_grad_kernel<T, false, U>;
+      fn<<<(unsigned)blocks + pad_ctas(capacity, sms), dim3(32 * warps, per_cta), 0, stream>>>(
+          static_cast<const T*>(dy), dys, span_of<T>(dy, dys, rows, cols), static_cast<const T*>(in), is,
+          span_of<T>(in, is, capacity, cols), (int)capacity, (int)cols, words, slot, source, weights, (int)rows, n,
+          static_cast<T*>(din), dis, dweights, blocks)));
   KM_CUDA(cudaGetLastError());
   return KM_OK;
 }
