@@ -132,13 +132,14 @@ combine_kernel(const T* in, long long is, Span<T> iin, int capacity, int d, int 
 
 // blockDim.x threads (whole warps) take a row, blockDim.y rows share a CTA; the dot products are joined over a row's warps, 32 entries at
 // a time.
+constexpr int kCombineGradThreads = 128;
 template <typename T, bool ALIGNED, int AT_ONCE>
-__global__ void __launch_bounds__(kMoveThreads)
+__global__ void __launch_bounds__(kCombineGradThreads, ALIGNED ? 10 : 6)
 combine_grad_kernel(const T* dy, long long dys, Span<T> gin, const T* in, long long is, Span<T> iin, int capacity, int d, int words,
                     const int* slot, const int* source, const float* weights, int rows, int n, T* din, long long dis, float* dweights,
                     int blocks) {
   constexpr int V = Piece<T>::V, H = V / 2;
-  __shared__ float red[kMoveThreads / 32][32];
+  __shared__ float red[kCombineGradThreads / 32][32];
   if ((int)blockIdx.x >= blocks) {
     zero_unused(din, dis, d, source, capacity, blockIdx.x - blocks, gridDim.x - blocks);
     return;
@@ -226,7 +227,7 @@ combine_grad_kernel(const T* dy, long long dys, Span<T> gin, const T* in, long l
 // (64 a processor), more for fewer rows.
 inline int combine_grad_warps(size_t rows, int words, int sms) {
   int w = 1;
-  while (w < kMoveThreads / 32 && (words + 31) / 32 > w && rows * w < (size_t)sms * 64) w *= 2;
+  while (w < kCombineGradThreads / 32 && (words + 31) / 32 > w && rows * w < (size_t)sms * 64) w *= 2;
   return w;
 }
 

@@ -271,6 +271,7 @@ int dispatch(int dtype, const void* x, long long xs, size_t rows, size_t cols, i
   do {                                                                                     \
     if ((n) == 1) { constexpr int U = 1; __VA_ARGS__; }                                    \
     else if ((n) == 2) { constexpr int U = 2; __VA_ARGS__; }                               \
+    else if ((n) == 3) { constexpr int U = 3; __VA_ARGS__; }                               \
     else { constexpr int U = 4; __VA_ARGS__; }                                             \
   } while (0)
 
@@ -309,7 +310,7 @@ int combine_grad(int dtype, const void* dy, long long dys, const void* in, long 
   KM_TRY(sm_count(&sms));
   const bool al = rows_aligned(dy, dys, rows, cols, size) && rows_aligned(in, is, capacity, cols, size) &&
                   rows_aligned(din, dis, capacity, cols, size);
-  const int words = move_words(cols, size, al), warps = combine_grad_warps(rows, words, sms), per_cta = kMoveThreads / 32 / warps;
+  const int words = move_words(cols, size, al), warps = combine_grad_warps(rows, words, sms), per_cta = kCombineGradThreads / 32 / warps;
   const int blocks = (int)((rows + per_cta - 1) / per_cta);
   KM_ROWS_DTYPE(dtype, T, KM_ROWS_AT_ONCE(n, U,
       const auto fn = al ? combine_grad_kernel<T, true, U> : combine_grad_kernel<T, false, U>;
