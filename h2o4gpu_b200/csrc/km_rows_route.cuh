@@ -7,13 +7,13 @@
 //   over the taken: ds = scale * weight (dweight - c) at the taken, 0 elsewhere;  over all: ds_e = scale * p_e (dweight_e - c)
 #pragma once
 
-#include "km_rows.cuh"
+#include "km_rows_vec.cuh"
 
 namespace km {
 namespace rows {
 
 constexpr int kRouteMax = 32;    // clusters a row can take
-constexpr int kRouteWarps = 8;
+constexpr int kRouteMaxK = 1 << 24;
 
 // A score as a number that orders: larger is better, 0 = cannot be taken.  (float bits of a positive number order as
 // integers, those of a negative one the other way round; the largest finite number maps below 0xffffffff.)
@@ -40,42 +40,272 @@ __device__ __forceinline__ unsigned long long warp_max_key(unsigned long long v)
   return v;
 }
 
-// One warp per row: n passes over the scores, each for the best key below the last one.
+
+// A score's quality: larger is better, -inf cannot be taken.
 template <typename T>
+__device__ __forceinline__ float route_value(T s, float sign) {
+  return fminf(fmaxf(sign * to_f(s), -INFINITY), 3.402823466e38f);      // (the maximum of NaN and a number is the number)
+}
+
+// Both kernels find the n best of a row without sorting it: the maxima of some groups of its scores give a bound that the n best reach
+// (the n-th largest of the maxima), and few scores besides them do.  Those are collected, and only they are put in order.
+
+// ---- one lane per row: scores that lie cluster after cluster, and rows too short for a warp ---------------------------------------------
+// `split` warps share the clusters of 32 rows, each a run of them.
+constexpr int kRouteGroup = 8;      // scores of a group, and loads on their way together
+constexpr int kRouteList = 16;      // collected scores of a lane
+
+// Puts (q, e) into a list of N sorted by descending quality; e is above all entries' clusters, so ties stay in front.
+template <int N>
+__device__ __forceinline__ void route_insert(float (&v)[N], int (&id)[N], float q, int e) {
+  if (!(q > v[N - 1])) return;
+#pragma unroll
+  for (int j = N - 1; j >= 0; --j) {
+    const bool here = q > v[j], above = j > 0 && q > v[j > 0 ? j - 1 : 0];
+    if (here) {      // everything from its place on moves down by one
+      v[j] = above ? v[j > 0 ? j - 1 : 0] : q;
+      id[j] = above ? id[j > 0 ? j - 1 : 0] : e;
+    }
+  }
+}
+// The same for values alone.
+template <int N>
+__device__ __forceinline__ void route_insert(float (&v)[N], float q) {
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    const float lo = fminf(v[j], q);
+    v[j] = fmaxf(v[j], q);
+    q = lo;
+  }
+}
+
+template <typename T, int N>
+__global__ void __launch_bounds__(512)
+route_lane_kernel(const T* s, long long rs, long long cs, int rows, int k, int n, float scale, bool over_all, int split, int* ids,
+                  float* weights, float* best, float* total) {
+  extern __shared__ float2 shared[];       // the lanes' lists, then what the warps of a tile tell each other
+  const int lane = threadIdx.x, warp = threadIdx.y, part = warp % split;
+  const long long tile = (long long)blockIdx.x * (blockDim.y / split) + warp / split;
+  const int t = (int)min(tile * 32 + lane, (long long)rows - 1);     // a lane behind the last row works on that row and writes nothing
+  const bool valid = tile * 32 + lane < rows;
+  const T* sr = s + t * rs;
+  const float sign = scale > 0.f ? 1.f : -1.f, a = fabsf(scale);
+  const int per = ((k + split - 1) / split + kRouteGroup - 1) / kRouteGroup * kRouteGroup;
+  const int c0 = min(k, part * per), c1 = min(k, c0 + per);
+  float v[N];
+  int id[N];
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    v[j] = -INFINITY;
+    id[j] = -1;
+  }
+  float first = -INFINITY, sum = 0.f;
+  // f(quality, cluster) over this warp's clusters, a group's loads together
+  const auto walk = [&](auto f, auto ends) {
+    for (int c = c0; c < c1; c += kRouteGroup) {
+      T raw[kRouteGroup];
+      if (c + kRouteGroup <= c1) {
+#pragma unroll
+        for (int u = 0; u < kRouteGroup; ++u) raw[u] = sr[(c + u) * cs];
+#pragma unroll
+        for (int u = 0; u < kRouteGroup; ++u) f(route_value(raw[u], sign), c + u);
+      } else {
+#pragma unroll
+        for (int u = 0; u < kRouteGroup; ++u)
+          if (c + u < c1) raw[u] = sr[(c + u) * cs];
+#pragma unroll
+        for (int u = 0; u < kRouteGroup; ++u)
+          if (c + u < c1) f(route_value(raw[u], sign), c + u);
+      }
+      ends();
+    }
+  };
+  // no bound to be had from one score, nor from fewer groups than are taken: one walk
+  const bool direct = N == 1 || k <= kRouteGroup * N;
+  if (direct) {
+    walk([&](float q, int e) { route_insert(v, id, q, e); }, [] {});
+    first = v[0];
+  } else {
+    float m[N], g = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < N; ++j) m[j] = -INFINITY;
+    walk([&](float q, int) { g = fmaxf(g, q); }, [&] { route_insert(m, g); g = -INFINITY; });
+    if (split > 1) {      // the bound of all the row's groups
+      float* told = reinterpret_cast<float*>(shared);
+#pragma unroll
+      for (int j = 0; j < N; ++j) told[(warp * N + j) * 32 + lane] = m[j];
+      __syncthreads();
+      for (int w = warp - part; w < warp - part + split; ++w)
+        if (w != warp)
+          for (int j = 0; j < N; ++j) route_insert(m, told[(w * N + j) * 32 + lane]);
+      __syncthreads();
+    }
+    first = m[0];
+    const float bound = fmaxf(m[N - 1], -3.402823466e38f);      // anything but -inf while fewer than N groups have one
+    float2* list = shared + (warp * 32 + lane);
+    const int stride = blockDim.y * 32;
+    int have = 0;
+    const auto put = [&] {
+      for (int i = 0; i < have; ++i) {
+        const float2 o = list[i * stride];
+        route_insert(v, id, o.x, __float_as_int(o.y));
+      }
+      have = 0;
+    };
+    walk([&](float q, int e) {
+      if (q >= bound) {
+        list[have * stride] = make_float2(q, __int_as_float(e));
+        if (++have == kRouteList) put();
+      }
+    }, [] {});
+    put();
+  }
+  if (split > 1) {       // the tile's first warp joins the others' lists, in the clusters' order
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < N; ++j) shared[(warp * N + j) * 32 + lane] = make_float2(v[j], __int_as_float(id[j]));
+    __syncthreads();
+    if (part == 0)
+      for (int w = warp + 1; w < warp + split; ++w)
+        for (int j = 0; j < N; ++j) {
+          const float2 o = shared[(w * N + j) * 32 + lane];
+          route_insert(v, id, o.x, __float_as_int(o.y));
+        }
+    if (direct) {       // what the sums below start from
+      __syncthreads();
+      if (part == 0) reinterpret_cast<float*>(shared)[warp * 32 + lane] = v[0];
+      __syncthreads();
+      first = reinterpret_cast<float*>(shared)[(warp - part) * 32 + lane];
+    }
+  }
+  const float q0 = first > -INFINITY ? first : 0.f;
+  if (over_all) {
+    walk([&](float q, int) { if (q > -INFINITY) sum += expf(a * (q - q0)); }, [] {});
+    if (split > 1) {
+      __syncthreads();
+      reinterpret_cast<float*>(shared)[warp * 32 + lane] = sum;
+      __syncthreads();
+      if (part == 0)
+        for (int w = warp + 1; w < warp + split; ++w) sum += reinterpret_cast<float*>(shared)[w * 32 + lane];
+    }
+  }
+  if (part != 0 || !valid) return;
+  float z[N];
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    z[j] = id[j] >= 0 ? expf(a * (v[j] - q0)) : 0.f;
+    if (!over_all && j < n) sum += z[j];
+  }
+#pragma unroll
+  for (int j = 0; j < N; ++j)
+    if (j < n) {
+      ids[(long long)t * n + j] = id[j];
+      weights[(long long)t * n + j] = id[j] >= 0 ? z[j] / sum : 0.f;
+    }
+  best[t] = sign * q0;
+  total[t] = sum;
+}
+
+// ---- one warp per row: scores that lie row after row ---------------------------------------------------------------------------------
+// The groups are the lanes.  HELD pieces of 16 bytes a lane stay in registers; 0: longer rows, read a second time (from L2).
+constexpr int kRouteWarps = 8;
+
+template <typename T, int HELD, bool ALIGNED>
 __global__ void __launch_bounds__(kRouteWarps * 32)
-route_kernel(const T* s, long long rs, long long cs, int rows, int k, int n, float scale, bool over_all, int* ids, float* weights,
-             float* best, float* total) {
-  const int lane = threadIdx.x & 31;
-  const int t = blockIdx.x * kRouteWarps + (threadIdx.x >> 5);
+route_warp_kernel(const T* s, long long rs, Span<T> in, int rows, int k, int n, float scale, bool over_all, int* ids, float* weights,
+                  float* best, float* total) {
+  constexpr int V = Piece<T>::V;
+  __shared__ unsigned long long lists[kRouteWarps][32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x / 32;
+  const int t = blockIdx.x * kRouteWarps + warp;
   if (t >= rows) return;
+  unsigned long long* list = lists[warp];
   const T* sr = s + (long long)t * rs;
   const float sign = scale > 0.f ? 1.f : -1.f, a = fabsf(scale);
-  unsigned long long last = ~0ULL, mine = 0ULL;
+  const int pieces = (k + V - 1) / V;
+  float held[HELD ? HELD : 1][V];
+  const auto values = [&](int i, float (&q)[V]) {      // piece i; -inf behind the row's end
+    const Piece<T> p = load_piece<T, ALIGNED>(sr, i, k, in);
+#pragma unroll
+    for (int e = 0; e < V; ++e) q[e] = i * V + e < k ? route_value(p.e[e], sign) : -INFINITY;
+  };
+  // f(qualities of a piece, piece) over the row; every lane makes the same number of calls
+  const auto walk = [&](auto f) {
+    if (HELD) {
+#pragma unroll
+      for (int h = 0; h < HELD; ++h) f(held[h], lane + h * 32);
+    } else {
+      for (int i0 = 0; i0 < pieces; i0 += 32) {
+        float q[V];
+        values(i0 + lane, q);
+        f(q, i0 + lane);
+      }
+    }
+  };
+#pragma unroll
+  for (int h = 0; h < HELD; ++h) values(lane + h * 32, held[h]);
+  float m = -INFINITY;
+  walk([&](const float (&q)[V], int) {
+#pragma unroll
+    for (int e = 0; e < V; ++e) m = fmaxf(m, q[e]);
+  });
+  // the n-th largest of the lanes' maxima
+  unsigned int o = route_order(m), top = 0, nth = 0;
   for (int j = 0; j < n; ++j) {
-    unsigned long long m = 0ULL;
-    for (int e = lane; e < k; e += 32) {
-      const unsigned long long key = route_key(sign * to_f(sr[e * cs]), e);
-      if (key < last && key > m) m = key;
-    }
-    m = warp_max_key(m);
-    if (lane == j) mine = m;
-    last = m;
+    const unsigned int w = __reduce_max_sync(0xffffffffu, o);
+    if (j == 0) top = w;
+    nth = w;
+    if (w == 0) break;
+    if (lane == __ffs(__ballot_sync(0xffffffffu, o == w)) - 1) o = 0;
   }
-  const float q = route_quality((unsigned int)(mine >> 32));
-  const float q0 = __shfl_sync(0xffffffffu, mine ? q : 0.f, 0);
-  const float z = mine ? expf(a * (q - q0)) : 0.f;
-  float sum = z;
-  if (over_all) {
-    sum = 0.f;
-    for (int e = lane; e < k; e += 32) {
-      const unsigned int o = route_order(sign * to_f(sr[e * cs]));
-      if (o) sum += expf(a * (route_quality(o) - q0));
+  const float q0 = top ? route_quality(top) : 0.f;
+  const float bound = nth ? route_quality(nth) : -3.402823466e38f;
+  int have = 0;
+  float sum = 0.f;
+  walk([&](const float (&q)[V], int i) {
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      const unsigned int reach = __ballot_sync(0xffffffffu, q[e] >= bound);
+      if (reach) {
+        const int at = have + __popc(reach & ((1u << lane) - 1u));
+        if (q[e] >= bound && at < 32) list[at] = route_key(q[e], i * V + e);
+        have += __popc(reach);
+      }
     }
+    if (over_all)
+#pragma unroll
+      for (int e = 0; e < V; ++e) sum += q[e] > -INFINITY ? expf(a * (q[e] - q0)) : 0.f;
+  });
+  __syncwarp();
+  // `mine`: this lane's score among the n best, `place` where it goes; lanes without one fill the places behind
+  unsigned long long mine = 0ULL;
+  int place = 0;
+  if (have <= 32) {
+    mine = lane < have ? list[lane] : 0ULL;
+    for (int i = 0; i < have; ++i) place += list[i] > mine;
+    if (lane >= have) place = lane;
+    if (place >= n) mine = 0ULL;
+  } else {      // more reach the bound (ties): the best one below the last, n times
+    unsigned long long last = ~0ULL;
+    for (int j = 0; j < n; ++j) {
+      unsigned long long b = 0ULL;
+      walk([&](const float (&q)[V], int i) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          const unsigned long long key = route_key(q[e], i * V + e);
+          if (key < last && key > b) b = key;
+        }
+      });
+      last = warp_max_key(b);
+      if (lane == j) mine = last;
+    }
+    place = lane;
   }
-  sum = warp_sum_f(sum);
-  if (lane < n) {
-    ids[(long long)t * n + lane] = mine ? (int)~(unsigned int)mine : -1;
-    weights[(long long)t * n + lane] = mine ? z / sum : 0.f;
+  const float z = mine ? expf(a * (route_quality((unsigned int)(mine >> 32)) - q0)) : 0.f;
+  sum = warp_sum_f(over_all ? sum : z);
+  if (place < n) {
+    ids[(long long)t * n + place] = mine ? (int)~(unsigned int)mine : -1;
+    weights[(long long)t * n + place] = mine ? z / sum : 0.f;
   }
   if (lane == 0) {
     best[t] = sign * q0;
@@ -83,12 +313,16 @@ route_kernel(const T* s, long long rs, long long cs, int rows, int k, int n, flo
   }
 }
 
-template <typename T>
+// ---- the gradient ----------------------------------------------------------------------------------------------------------------------
+// Every score's own part first (zero over the taken alone), then the taken ones' over it.
+
+// One warp per row, 16-byte pieces.
+template <typename T, bool ALIGNED>
 __global__ void __launch_bounds__(kRouteWarps * 32)
-route_grad_kernel(const float* dweights, const T* s, long long rs, long long cs, int rows, int k, int n, float scale, bool over_all,
-                  const int* ids, const float* weights, const float* best, const float* total, T* ds, long long drs, long long dcs) {
-  const int lane = threadIdx.x & 31;
-  const int t = blockIdx.x * kRouteWarps + (threadIdx.x >> 5);
+route_grad_warp_kernel(const float* dweights, const T* s, long long rs, Span<T> in, int rows, int k, int n, float scale, bool over_all,
+                       const int* ids, const float* weights, const float* best, const float* total, T* ds, long long drs) {
+  constexpr int V = Piece<T>::V, H = V / 2;
+  const int lane = threadIdx.x & 31, t = blockIdx.x * kRouteWarps + threadIdx.x / 32;
   if (t >= rows) return;
   int id = -1;
   float w = 0.f, g = 0.f;
@@ -96,29 +330,134 @@ route_grad_kernel(const float* dweights, const T* s, long long rs, long long cs,
     id = ids[(long long)t * n + lane];
     w = weights[(long long)t * n + lane];
     g = dweights[(long long)t * n + lane];
-    if (id < 0 || id >= k) { id = -1; w = 0.f; g = 0.f; }
   }
-  const float c = warp_sum_f(id >= 0 ? w * g : 0.f);
+  const bool taken = id >= 0 && id < k;
+  const float c = warp_sum_f(taken ? w * g : 0.f);
   T* dr = ds + (long long)t * drs;
+  const T* sr = over_all ? s + (long long)t * rs : nullptr;
   const float sign = scale > 0.f ? 1.f : -1.f, a = fabsf(scale);
-  const float q0 = over_all ? sign * best[t] : 0.f, sum = over_all ? total[t] : 0.f;
-  for (int e0 = 0; e0 < k; e0 += 32) {
-    const int e = e0 + lane;
-    float ge = 0.f, we = 0.f;
-    bool taken = false;
-    for (int j = 0; j < n; ++j) {
-      const int idj = __shfl_sync(0xffffffffu, id, j);
-      const float gj = __shfl_sync(0xffffffffu, g, j), wj = __shfl_sync(0xffffffffu, w, j);
-      if (idj == e) { taken = true; ge = gj; we = wj; }
-    }
-    if (e >= k) continue;
-    float v = taken ? scale * we * (ge - c) : 0.f;
+  const float sum = over_all ? total[t] : 0.f, q0 = over_all ? sign * best[t] : 0.f, f = sum > 0.f ? -scale * c / sum : 0.f;
+  const int pieces = ((k + V - 1) / V + 31) / 32 * 32;
+  for (int i = lane; i < pieces; i += 32) {
+    Piece<T> p;
+    p.q = make_uint4(0u, 0u, 0u, 0u);
     if (over_all) {
-      const unsigned int o = route_order(sign * to_f(s[(long long)t * rs + e * cs]));
-      v = o && sum > 0.f ? scale * (expf(a * (route_quality(o) - q0)) / sum) * (ge - c) : 0.f;
+      p = load_piece<T, ALIGNED>(sr, i, k, in);
+      float2 o[H];
+#pragma unroll
+      for (int e = 0; e < H; ++e) {
+        const float qx = route_value(p.e[2 * e], sign), qy = route_value(p.e[2 * e + 1], sign);
+        o[e] = make_float2(qx > -INFINITY ? f * expf(a * (qx - q0)) : 0.f, qy > -INFINITY ? f * expf(a * (qy - q0)) : 0.f);
+      }
+      p = pack<T>(o);
+    }
+    store_piece<T, ALIGNED>(dr, i, k, p);
+  }
+  __syncwarp();
+  if (taken) dr[id] = from_f<T>(scale * w * (g - c));
+}
+
+// One thread per row and run of clusters: scores that lie cluster after cluster, or in other strides.
+constexpr int kRouteGradThreads = 128;
+template <typename T>
+__global__ void __launch_bounds__(kRouteGradThreads)
+route_grad_lane_kernel(const float* dweights, const T* s, long long rs, long long cs, int rows, int k, int per, int n, float scale,
+                       bool over_all, const int* ids, const float* weights, const float* best, const float* total, T* ds, long long drs,
+                       long long dcs) {
+  const long long at = (long long)blockIdx.x * kRouteGradThreads + threadIdx.x;
+  if (at >= rows) return;
+  const int t = (int)at, c0 = blockIdx.y * per, c1 = min(k, c0 + per);
+  float c = 0.f;
+  for (int j = 0; j < n; ++j) {
+    const int id = ids[(long long)t * n + j];
+    if (id >= 0 && id < k) c = fmaf(weights[(long long)t * n + j], dweights[(long long)t * n + j], c);
+  }
+  const float sign = scale > 0.f ? 1.f : -1.f, a = fabsf(scale);
+  const float sum = over_all ? total[t] : 0.f, q0 = over_all ? sign * best[t] : 0.f, f = sum > 0.f ? -scale * c / sum : 0.f;
+  const T* sr = s + t * rs;
+  T* dr = ds + t * drs;
+#pragma unroll 8
+  for (int e = c0; e < c1; ++e) {
+    float v = 0.f;
+    if (over_all) {
+      const float q = route_value(sr[e * cs], sign);
+      if (q > -INFINITY) v = f * expf(a * (q - q0));
     }
     dr[e * dcs] = from_f<T>(v);
   }
+  for (int j = 0; j < n; ++j) {
+    const int id = ids[(long long)t * n + j];
+    if (id >= c0 && id < c1) dr[id * dcs] = from_f<T>(scale * weights[(long long)t * n + j] * (dweights[(long long)t * n + j] - c));
+  }
+}
+
+// ---- launches --------------------------------------------------------------------------------------------------------------------------
+
+template <typename T>
+int route_launch(const T* s, long long rs, long long cs, int rows, int k, int n, float scale, bool over_all, int* ids, float* weights,
+                 float* best, float* total, int sms, cudaStream_t stream) {
+  // a lane per row where lanes' loads lie side by side, or a row is no longer than the line that its lane's loads share
+  if (cs != 1 || (size_t)k * sizeof(T) <= 128 || (rs == 1 && rows > 1)) {
+    const long long tiles = ((long long)rows + 31) / 32;
+    int most = 16;
+    while (most * n > 128) most /= 2;       // the lists that the warps of a tile exchange: 32 KB
+    int split = 1;
+    while (split < most && tiles * split < (long long)sms * 16 && k / split >= 64) split *= 2;
+    const int warps = std::max(4, split), per_cta = warps / split;
+    const auto launch = [&](auto count) -> int {
+      constexpr int N = count();
+      const size_t smem = sizeof(float2) * 32 * warps * std::max(N == 1 ? 1 : kRouteList, split > 1 ? N : 1);
+      const auto fn = route_lane_kernel<T, N>;
+      KM_CUDA(allow_smem(fn, smem));
+      fn<<<(unsigned)((tiles + per_cta - 1) / per_cta), dim3(32, warps), smem, stream>>>(s, rs, cs, rows, k, n, scale, over_all, split,
+                                                                                       ids, weights, best, total);
+      KM_CUDA(cudaGetLastError());
+      return KM_OK;
+    };
+    using std::integral_constant;
+    if (n == 1) return launch(integral_constant<int, 1>());
+    if (n == 2) return launch(integral_constant<int, 2>());
+    if (n <= 4) return launch(integral_constant<int, 4>());
+    if (n <= 8) return launch(integral_constant<int, 8>());
+    if (n <= 16) return launch(integral_constant<int, 16>());
+    return launch(integral_constant<int, 32>());
+  }
+  const bool al = rows_aligned(s, rs, rows, k, sizeof(T));
+  const int pieces = (k + Piece<T>::V - 1) / Piece<T>::V;
+  const auto pick = [&](auto aligned_) {
+    constexpr bool AL = aligned_();
+    return pieces <= 32 ? route_warp_kernel<T, 1, AL> : pieces <= 64 ? route_warp_kernel<T, 2, AL>
+         : pieces <= 128 ? route_warp_kernel<T, 4, AL> : route_warp_kernel<T, 0, AL>;
+  };
+  const auto fn = al ? pick(std::true_type()) : pick(std::false_type());
+  fn<<<(rows + kRouteWarps - 1) / kRouteWarps, kRouteWarps * 32, 0, stream>>>(s, rs, span_of<T>(s, rs, rows, k), rows, k, n, scale,
+                                                                            over_all, ids, weights, best, total);
+  KM_CUDA(cudaGetLastError());
+  return KM_OK;
+}
+
+template <typename T>
+int route_grad_launch(const float* dweights, const T* s, long long rs, long long cs, int rows, int k, int n, float scale, bool over_all,
+                      const int* ids, const float* weights, const float* best, const float* total, T* ds, long long drs, long long dcs,
+                      int sms, cudaStream_t stream) {
+  if (dcs == 1 && (!over_all || cs == 1)) {
+    const bool al = rows_aligned(ds, drs, rows, k, sizeof(T)) && (!over_all || rows_aligned(s, rs, rows, k, sizeof(T)));
+    const auto fn = al ? route_grad_warp_kernel<T, true> : route_grad_warp_kernel<T, false>;
+    fn<<<(rows + kRouteWarps - 1) / kRouteWarps, kRouteWarps * 32, 0, stream>>>(
+        dweights, s, rs, over_all ? span_of<T>(s, rs, rows, k) : Span<T>{nullptr, nullptr}, rows, k, n, scale, over_all, ids, weights,
+        best, total, ds, drs);
+    KM_CUDA(cudaGetLastError());
+    return KM_OK;
+  }
+  // runs of clusters so long that a row's own values are read rarely, and enough of them to fill the device
+  const long long tiles = ((long long)rows + kRouteGradThreads - 1) / kRouteGradThreads;
+  int runs = 1;
+  while (runs < 1024 && tiles * runs < (long long)sms * 16 && k / runs > 16) runs *= 2;
+  const int per = (k + runs - 1) / runs;
+  route_grad_lane_kernel<T><<<dim3((unsigned)tiles, (k + per - 1) / per), kRouteGradThreads, 0, stream>>>(
+      dweights, s, rs, cs, rows, k, per, n, scale, over_all, ids, weights, best, total, ds, drs, dcs);
+  KM_CUDA(cudaGetLastError());
+  return KM_OK;
 }
 
 }  // namespace rows

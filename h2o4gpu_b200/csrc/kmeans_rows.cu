@@ -135,7 +135,7 @@ bool strides_ok(long long rs, long long cs) { return rs >= 0 && cs >= 0 && rs <=
 
 int check_route(const char* name, int dtype, size_t rows, int k, int n, float scale) {
   if (!elem_size(dtype)) KM_FAIL(KM_EINVAL, std::string(name) + ": scores are float32, float16 or bfloat16");
-  if (rows > kMaxRows || k < 1) KM_FAIL(KM_EINVAL, std::string(name) + ": bad argument");
+  if (rows > kMaxRows || k < 1 || k > kRouteMaxK) KM_FAIL(KM_EINVAL, std::string(name) + ": bad argument");
   if (n < 1 || n > kRouteMax || n > k)
     KM_FAIL(KM_EINVAL, std::string(name) + ": a row takes 1 to " + std::to_string(kRouteMax) + " clusters, and no more than there are");
   if (!std::isfinite(scale) || scale == 0.f) KM_FAIL(KM_EINVAL, std::string(name) + ": scale must be finite and not zero");
@@ -149,11 +149,12 @@ int route(int dtype, const void* scores, long long rs, long long cs, size_t rows
   if (!scores || !aligned(scores, elem_size(dtype)) || !strides_ok(rs, cs) || !ids || !weights || !best || !total ||
       !aligned(ids, 4) || !aligned(weights, 4) || !aligned(best, 4) || !aligned(total, 4))
     KM_FAIL(KM_EINVAL, "kmeans_route: bad argument");
+  int sms = 0, rc = KM_OK;
+  KM_TRY(sm_count(&sms));
   KM_ROWS_DTYPE(dtype, T,
-      route_kernel<T><<<(unsigned)((rows + kRouteWarps - 1) / kRouteWarps), kRouteWarps * 32, 0, stream>>>(
-          static_cast<const T*>(scores), rs, cs, (int)rows, k, n, scale, over_all != 0, ids, weights, best, total));
-  KM_CUDA(cudaGetLastError());
-  return KM_OK;
+      rc = route_launch<T>(static_cast<const T*>(scores), rs, cs, (int)rows, k, n, scale, over_all != 0, ids, weights, best, total, sms,
+                           stream));
+  return rc;
 }
 
 int route_grad(int dtype, const float* dweights, const void* scores, long long rs, long long cs, size_t rows, int k, int n,
@@ -169,12 +170,12 @@ int route_grad(int dtype, const float* dweights, const void* scores, long long r
     KM_FAIL(KM_EINVAL, "kmeans_route_grad: weights over all clusters need the scores, best and total");
   if (!((dcs == 1 && (drs >= k || rows == 1)) || (drs == 1 && (dcs >= (long long)rows || k == 1))))
     KM_FAIL(KM_EINVAL, "kmeans_route_grad: dscores must lie row after row or cluster after cluster");
+  int sms = 0, rc = KM_OK;
+  KM_TRY(sm_count(&sms));
   KM_ROWS_DTYPE(dtype, T,
-      route_grad_kernel<T><<<(unsigned)((rows + kRouteWarps - 1) / kRouteWarps), kRouteWarps * 32, 0, stream>>>(
-          dweights, static_cast<const T*>(scores), rs, cs, (int)rows, k, n, scale, over_all != 0, ids, weights, best, total,
-          static_cast<T*>(dscores), drs, dcs));
-  KM_CUDA(cudaGetLastError());
-  return KM_OK;
+      rc = route_grad_launch<T>(dweights, static_cast<const T*>(scores), rs, cs, (int)rows, k, n, scale, over_all != 0, ids, weights,
+                                best, total, static_cast<T*>(dscores), drs, dcs, sms, stream));
+  return rc;
 }
 
 int check_sort(const char* name, size_t rows, int n, int k, int align, size_t* capacity) {

@@ -319,7 +319,7 @@ int kmeans_layer_norm_grad(int dtype, const void* dy, long long dy_stride, const
                            int param_dtype, void* dx, long long dx_stride, float* dweight, float* dbias,
                            void* workspace, size_t workspace_bytes, void* stream);
 
-/* The n best clusters of each row (1 <= n <= min(k, 32)) and their weights.  scores[row * row_stride + cluster *
+/* The n best clusters of each row (1 <= n <= min(k, 32), k <= 2^24) and their weights.  scores[row * row_stride + cluster *
  * col_stride]: distances in transform's column-major layout (row_stride 1), or a linear router's row-major
  * logits (col_stride 1); other strides work too.  scale > 0: larger scores are better; scale < 0: smaller ones
  * (distances; scale = -1 / temperature).  Ties go to the lowest cluster; NaN and infinitely bad scores are never
