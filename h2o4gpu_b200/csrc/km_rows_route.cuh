@@ -47,6 +47,15 @@ __device__ __forceinline__ float route_value(T s, float sign) {
   return fminf(fmaxf(sign * to_f(s), -INFINITY), 3.402823466e38f);      // (the maximum of NaN and a number is the number)
 }
 
+// exp(x), x <= 0, for sums of many terms: 2^(x log2 e) with the product rounded once more than in expf, which puts |x| 2^-24 of a term
+// on top - at most 0.4 2^-24 of the largest one, as x e^-x is - for a third of the instructions.
+__device__ __forceinline__ float exp2_fast(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+constexpr float kLog2E = 1.44269504f;
+
 // Both kernels find the n best of a row without sorting it: the maxima of some groups of its scores give a bound that the n best reach
 // (the n-th largest of the maxima), and few scores besides them do.  Those are collected, and only they are put in order.
 
@@ -100,22 +109,23 @@ route_lane_kernel(const T* s, long long rs, long long cs, int rows, int k, int n
     id[j] = -1;
   }
   float first = -INFINITY, sum = 0.f;
-  // f(quality, cluster) over this warp's clusters, a group's loads together
+  // f(score, cluster) over this warp's clusters, a group's loads together; then ends() of the group
   const auto walk = [&](auto f, auto ends) {
+    const T* p = sr + c0 * cs;
     for (int c = c0; c < c1; c += kRouteGroup) {
       T raw[kRouteGroup];
       if (c + kRouteGroup <= c1) {
 #pragma unroll
-        for (int u = 0; u < kRouteGroup; ++u) raw[u] = sr[(c + u) * cs];
+        for (int u = 0; u < kRouteGroup; ++u, p += cs) raw[u] = *p;
 #pragma unroll
-        for (int u = 0; u < kRouteGroup; ++u) f(route_value(raw[u], sign), c + u);
+        for (int u = 0; u < kRouteGroup; ++u) f(raw[u], c + u);
       } else {
 #pragma unroll
         for (int u = 0; u < kRouteGroup; ++u)
-          if (c + u < c1) raw[u] = sr[(c + u) * cs];
+          if (c + u < c1) raw[u] = p[u * cs];
 #pragma unroll
         for (int u = 0; u < kRouteGroup; ++u)
-          if (c + u < c1) f(route_value(raw[u], sign), c + u);
+          if (c + u < c1) f(raw[u], c + u);
       }
       ends();
     }
@@ -123,13 +133,14 @@ route_lane_kernel(const T* s, long long rs, long long cs, int rows, int k, int n
   // no bound to be had from one score, nor from fewer groups than are taken: one walk
   const bool direct = N == 1 || k <= kRouteGroup * N;
   if (direct) {
-    walk([&](float q, int e) { route_insert(v, id, q, e); }, [] {});
+    walk([&](T r, int e) { route_insert(v, id, route_value(r, sign), e); }, [] {});
     first = v[0];
   } else {
     float m[N], g = -INFINITY;
 #pragma unroll
     for (int j = 0; j < N; ++j) m[j] = -INFINITY;
-    walk([&](float q, int) { g = fmaxf(g, q); }, [&] { route_insert(m, g); g = -INFINITY; });
+    walk([&](T r, int) { g = fmaxf(g, sign * to_f(r)); },      // (which leaves NaN out)
+         [&] { route_insert(m, fminf(g, 3.402823466e38f)); g = -INFINITY; });
     if (split > 1) {      // the bound of all the row's groups
       float* told = reinterpret_cast<float*>(shared);
 #pragma unroll
@@ -152,12 +163,10 @@ route_lane_kernel(const T* s, long long rs, long long cs, int rows, int k, int n
       }
       have = 0;
     };
-    walk([&](float q, int e) {
-      if (q >= bound) {
-        list[have * stride] = make_float2(q, __int_as_float(e));
-        if (++have == kRouteList) put();
-      }
-    }, [] {});
+    walk([&](T r, int e) {
+      const float q = sign * to_f(r);
+      if (q >= bound) list[have++ * stride] = make_float2(fminf(q, 3.402823466e38f), __int_as_float(e));
+    }, [&] { if (have > kRouteList - kRouteGroup) put(); });
     put();
   }
   if (split > 1) {       // the tile's first warp joins the others' lists, in the clusters' order
@@ -180,7 +189,8 @@ route_lane_kernel(const T* s, long long rs, long long cs, int rows, int k, int n
   }
   const float q0 = first > -INFINITY ? first : 0.f;
   if (over_all) {
-    walk([&](float q, int) { if (q > -INFINITY) sum += expf(a * (q - q0)); }, [] {});
+    const float a2 = a * kLog2E;
+    walk([&](T r, int) { sum += exp2_fast(a2 * (route_value(r, sign) - q0)); }, [] {});
     if (split > 1) {
       __syncthreads();
       reinterpret_cast<float*>(shared)[warp * 32 + lane] = sum;
@@ -223,34 +233,44 @@ route_warp_kernel(const T* s, long long rs, Span<T> in, int rows, int k, int n, 
   const T* sr = s + (long long)t * rs;
   const float sign = scale > 0.f ? 1.f : -1.f, a = fabsf(scale);
   const int pieces = (k + V - 1) / V;
-  float held[HELD ? HELD : 1][V];
-  const auto values = [&](int i, float (&q)[V]) {      // piece i; -inf behind the row's end
-    const Piece<T> p = load_piece<T, ALIGNED>(sr, i, k, in);
+  const int per_lane = (pieces + 31) / 32;
+  const T none = from_f<T>(-sign * INFINITY);
+  const auto piece = [&](int i) {      // behind the row's end: scores that cannot be taken
+    Piece<T> p = load_piece<T, ALIGNED>(sr, i, k, in);
+    if ((i + 1) * V > k)
 #pragma unroll
-    for (int e = 0; e < V; ++e) q[e] = i * V + e < k ? route_value(p.e[e], sign) : -INFINITY;
+      for (int e = 0; e < V; ++e)
+        if (i * V + e >= k) p.e[e] = none;
+    return p;
   };
-  // f(qualities of a piece, piece) over the row; every lane makes the same number of calls
+  Piece<T> held[HELD ? HELD : 1];
+#pragma unroll
+  for (int h = 0; h < HELD; ++h) held[h] = piece(lane + h * 32);
+  // f(a piece's signed scores, piece) over the row; every lane makes the same number of calls
   const auto walk = [&](auto f) {
+    const auto call = [&](const Piece<T>& p, int i) {
+      float2 q[V / 2];
+      unpack(p, q);
+#pragma unroll
+      for (int e = 0; e < V / 2; ++e) q[e] = mul2(q[e], both(sign));
+      f(q, i);
+    };
     if (HELD) {
 #pragma unroll
-      for (int h = 0; h < HELD; ++h) f(held[h], lane + h * 32);
+      for (int h = 0; h < HELD; ++h) call(held[h], lane + h * 32);
     } else {
-      for (int i0 = 0; i0 < pieces; i0 += 32) {
-        float q[V];
-        values(i0 + lane, q);
-        f(q, i0 + lane);
-      }
+#pragma unroll 2
+      for (int i = lane; i < per_lane * 32; i += 32) call(piece(i), i);
     }
   };
-#pragma unroll
-  for (int h = 0; h < HELD; ++h) values(lane + h * 32, held[h]);
   float m = -INFINITY;
-  walk([&](const float (&q)[V], int) {
+  walk([&](const float2 (&q)[V / 2], int) {
 #pragma unroll
-    for (int e = 0; e < V; ++e) m = fmaxf(m, q[e]);
+    for (int e = 0; e < V / 2; ++e) m = fmaxf(m, fmaxf(q[e].x, q[e].y));      // (which leaves NaN out)
   });
   // the n-th largest of the lanes' maxima
-  unsigned int o = route_order(m), top = 0, nth = 0;
+  const unsigned int own = route_order(m);
+  unsigned int o = own, top = 0, nth = 0;
   for (int j = 0; j < n; ++j) {
     const unsigned int w = __reduce_max_sync(0xffffffffu, o);
     if (j == 0) top = w;
@@ -260,22 +280,35 @@ route_warp_kernel(const T* s, long long rs, Span<T> in, int rows, int k, int n, 
   }
   const float q0 = top ? route_quality(top) : 0.f;
   const float bound = nth ? route_quality(nth) : -3.402823466e38f;
+  // Only lanes whose maximum reaches the bound have scores that do: n of them, but for ties.  The warp looks through one such lane's
+  // scores after the other (they come from L1).
   int have = 0;
-  float sum = 0.f;
-  walk([&](const float (&q)[V], int i) {
-#pragma unroll
-    for (int e = 0; e < V; ++e) {
-      const unsigned int reach = __ballot_sync(0xffffffffu, q[e] >= bound);
-      if (reach) {
-        const int at = have + __popc(reach & ((1u << lane) - 1u));
-        if (q[e] >= bound && at < 32) list[at] = route_key(q[e], i * V + e);
-        have += __popc(reach);
-      }
+  for (unsigned int lanes = __ballot_sync(0xffffffffu, own >= max(nth, 1u)); lanes; lanes &= lanes - 1) {
+    const int l = __ffs(lanes) - 1;
+    for (int u0 = 0; u0 < per_lane * V; u0 += 32) {
+      const int u = u0 + lane, e = (l + u / V * 32) * V + u % V;
+      const float q = u < per_lane * V && e < k ? sign * to_f(sr[e]) : -INFINITY;
+      const unsigned int reach = __ballot_sync(0xffffffffu, q >= bound);
+      const int at = have + __popc(reach & ((1u << lane) - 1u));
+      if (q >= bound && at < 32) list[at] = route_key(q, e);
+      have += __popc(reach);
     }
-    if (over_all)
+  }
+  float sum = 0.f;
+  if (over_all) {
+    const float2 a2 = both(a * kLog2E), off = both(-q0);
+    float2 s2 = both(0.f);
+    const bool huge = q0 == 3.402823466e38f;      // perhaps an infinite one, which counts as this
+    walk([&](float2 (&q)[V / 2], int) {
 #pragma unroll
-      for (int e = 0; e < V; ++e) sum += q[e] > -INFINITY ? expf(a * (q[e] - q0)) : 0.f;
-  });
+      for (int e = 0; e < V / 2; ++e) {
+        if (huge) q[e] = make_float2(fminf(fmaxf(q[e].x, -INFINITY), q0), fminf(fmaxf(q[e].y, -INFINITY), q0));
+        const float2 x = mul2(a2, add2(q[e], off));
+        s2 = add2(s2, make_float2(exp2_fast(fmaxf(x.x, -INFINITY)), exp2_fast(fmaxf(x.y, -INFINITY))));
+      }
+    });
+    sum = s2.x + s2.y;
+  }
   __syncwarp();
   // `mine`: this lane's score among the n best, `place` where it goes; lanes without one fill the places behind
   unsigned long long mine = 0ULL;
@@ -289,10 +322,10 @@ route_warp_kernel(const T* s, long long rs, Span<T> in, int rows, int k, int n, 
     unsigned long long last = ~0ULL;
     for (int j = 0; j < n; ++j) {
       unsigned long long b = 0ULL;
-      walk([&](const float (&q)[V], int i) {
+      walk([&](const float2 (&q)[V / 2], int i) {
 #pragma unroll
         for (int e = 0; e < V; ++e) {
-          const unsigned long long key = route_key(q[e], i * V + e);
+          const unsigned long long key = route_key(e & 1 ? q[e / 2].y : q[e / 2].x, i * V + e);
           if (key < last && key > b) b = key;
         }
       });
