@@ -130,9 +130,7 @@ route_lane_kernel(const T* s, long long rs, long long cs, int rows, int k, int n
       ends();
     }
   };
-  // no bound to be had from one score, nor from fewer groups than are taken: one walk
-  const bool direct = N == 1 || k <= kRouteGroup * N;
-  if (direct) {
+  if (N == 1) {
     walk([&](T r, int e) { route_insert(v, id, route_value(r, sign), e); }, [] {});
     first = v[0];
   } else {
@@ -180,7 +178,7 @@ route_lane_kernel(const T* s, long long rs, long long cs, int rows, int k, int n
           const float2 o = shared[(w * N + j) * 32 + lane];
           route_insert(v, id, o.x, __float_as_int(o.y));
         }
-    if (direct) {       // what the sums below start from
+    if (N == 1) {       // what the sums below start from
       __syncthreads();
       if (part == 0) reinterpret_cast<float*>(shared)[warp * 32 + lane] = v[0];
       __syncthreads();
@@ -220,9 +218,10 @@ route_lane_kernel(const T* s, long long rs, long long cs, int rows, int k, int n
 // The groups are the lanes.  HELD pieces of 16 bytes a lane stay in registers; 0: longer rows, read a second time (from L2).
 constexpr int kRouteWarps = 8;
 
-template <typename T, int HELD, bool ALIGNED>
+enum RouteRows { kAligned, kUnaligned, kStrided };
+template <typename T, int HELD, RouteRows LIE>
 __global__ void __launch_bounds__(kRouteWarps * 32)
-route_warp_kernel(const T* s, long long rs, Span<T> in, int rows, int k, int n, float scale, bool over_all, int* ids, float* weights,
+route_warp_kernel(const T* s, long long rs, long long cs, Span<T> in, int rows, int k, int n, float scale, bool over_all, int* ids, float* weights,
                   float* best, float* total) {
   constexpr int V = Piece<T>::V;
   __shared__ unsigned long long lists[kRouteWarps][32];
@@ -236,11 +235,14 @@ route_warp_kernel(const T* s, long long rs, Span<T> in, int rows, int k, int n, 
   const int per_lane = (pieces + 31) / 32;
   const T none = from_f<T>(-sign * INFINITY);
   const auto piece = [&](int i) {      // behind the row's end: scores that cannot be taken
-    Piece<T> p = load_piece<T, ALIGNED>(sr, i, k, in);
-    if ((i + 1) * V > k)
+    Piece<T> p;
+    if (LIE != kStrided) p = load_piece<T, LIE == kAligned>(sr, i, k, in);
+    if (LIE == kStrided || (i + 1) * V > k)
 #pragma unroll
-      for (int e = 0; e < V; ++e)
+      for (int e = 0; e < V; ++e) {
         if (i * V + e >= k) p.e[e] = none;
+        else if (LIE == kStrided) p.e[e] = sr[(i * V + e) * cs];
+      }
     return p;
   };
   Piece<T> held[HELD ? HELD : 1];
@@ -287,7 +289,7 @@ route_warp_kernel(const T* s, long long rs, Span<T> in, int rows, int k, int n, 
     const int l = __ffs(lanes) - 1;
     for (int u0 = 0; u0 < per_lane * V; u0 += 32) {
       const int u = u0 + lane, e = (l + u / V * 32) * V + u % V;
-      const float q = u < per_lane * V && e < k ? sign * to_f(sr[e]) : -INFINITY;
+      const float q = u < per_lane * V && e < k ? sign * to_f(sr[LIE == kStrided ? e * cs : e]) : -INFINITY;
       const unsigned int reach = __ballot_sync(0xffffffffu, q >= bound);
       const int at = have + __popc(reach & ((1u << lane) - 1u));
       if (q >= bound && at < 32) list[at] = route_key(q, e);
@@ -344,6 +346,243 @@ route_warp_kernel(const T* s, long long rs, Span<T> in, int rows, int k, int n, 
     best[t] = sign * q0;
     total[t] = sum;
   }
+}
+
+// ---- one lane per row, the scores of 32 rows in shared memory --------------------------------------------------------------------------
+// What a row costs besides its scores is then paid once for 32 rows, and a lane can go back to the few groups that hold its n best - the n
+// with the largest maxima, ties to the lower: any other score comes behind n of those maxima.  `split` warps share a tile, each a
+// run of its groups; the warps then tell each other a bound and join their lists.
+//   BY_ROW: row r at r * stride bytes (an odd number of 16-byte words: lanes read those without bank conflicts); a group is 8 scores of it
+//   else:   cluster e's 32 scores at e * 32
+constexpr size_t kRouteTileBytes = 100 << 10;      // two CTAs a processor
+template <typename T>
+struct RouteTile {
+  static constexpr int G = kRouteGroup, WORDS = G * (int)sizeof(T) / 16;      // 16-byte words of a group
+  static int groups(int k) { return (k + G - 1) / G; }
+  static int stride(int k) { return (groups(k) * WORDS | 1) * 16; }
+  static size_t bytes(int k, bool by_row) { return by_row ? (size_t)32 * stride(k) : (size_t)groups(k) * G * 32 * sizeof(T); }
+};
+
+// Into a list of N sorted by descending quality, ties by cluster.
+template <int N>
+__device__ __forceinline__ void route_insert_tied(float (&v)[N], int (&id)[N], float q, int e) {
+  const auto before = [&](int j) { return q > v[j] || (q == v[j] && e < id[j]); };
+  if (!before(N - 1)) return;
+#pragma unroll
+  for (int j = N - 1; j >= 0; --j) {
+    const bool here = before(j), above = j > 0 && before(j > 0 ? j - 1 : 0);
+    if (here) {
+      v[j] = above ? v[j > 0 ? j - 1 : 0] : q;
+      id[j] = above ? id[j > 0 ? j - 1 : 0] : e;
+    }
+  }
+}
+
+template <typename T, int N, bool BY_ROW>
+__global__ void __launch_bounds__(512)
+route_tile_kernel(const T* s, long long rs, long long cs, int rows, int k, int n, float scale, bool over_all, int split, int tile_bytes,
+                  int* ids, float* weights, float* best, float* total) {
+  using Tile = RouteTile<T>;
+  constexpr int G = Tile::G, WORDS = Tile::WORDS, V = Piece<T>::V;
+  extern __shared__ uint4 tiles[];
+  const int lane = threadIdx.x, warp = threadIdx.y, part = warp % split, per_cta = blockDim.y / split;
+  const long long row0 = ((long long)blockIdx.x * per_cta + warp / split) * 32;
+  unsigned char* tile = reinterpret_cast<unsigned char*>(tiles) + (size_t)(warp / split) * tile_bytes;
+  float2* shared = reinterpret_cast<float2*>(reinterpret_cast<unsigned char*>(tiles) + (size_t)per_cta * tile_bytes);
+  const int here = (int)max(0LL, min(32LL, rows - row0));     // rows of the tile
+  const int groups = (k + G - 1) / G, stride = (groups * WORDS | 1) * 16;
+  const float sign = scale > 0.f ? 1.f : -1.f, a = fabsf(scale);
+  const T none = from_f<T>(-sign * INFINITY);
+  T* flat = reinterpret_cast<T*>(tile);
+  if (BY_ROW) {
+    const int words = k / V;      // the rows are whole words
+    for (int r = part; r < here; r += split) {
+      const uint4* from = reinterpret_cast<const uint4*>(s + (row0 + r) * rs);
+      uint4* to = reinterpret_cast<uint4*>(tile + (size_t)r * stride);
+      for (int i = lane; i < words; i += 32) copy_async(to + i, from + i);
+      for (int e = k + lane; e < groups * G; e += 32) reinterpret_cast<T*>(to)[e] = none;
+    }
+  } else {
+    constexpr int PER = 32 * (int)sizeof(T) / 16, AT_ONCE = 32 / PER;      // words of a cluster's 32 scores, clusters a step
+    if (here == 32) {
+      const T* from = s + row0 + lane % PER * V;
+      uint4* to = reinterpret_cast<uint4*>(tile) + lane;
+      for (int e = part * AT_ONCE + lane / PER; e < k; e += split * AT_ONCE)
+        copy_async(to + (e - lane / PER) * PER, reinterpret_cast<const uint4*>(from + e * cs));
+    } else if (lane < here) {
+      for (int e = part; e < k; e += split) flat[e * 32 + lane] = s[row0 + lane + e * cs];
+    }
+    for (int e = k + part; e < groups * G; e += split) flat[e * 32 + lane] = none;
+  }
+  copies_commit();
+  copies_wait<0>();
+  __syncthreads();
+
+  // the signed scores of a group
+  const auto group = [&](int g, float2 (&q)[G / 2]) {
+    if (BY_ROW) {
+      const uint4* w = reinterpret_cast<const uint4*>(tile + (size_t)lane * stride) + g * WORDS;
+#pragma unroll
+      for (int i = 0; i < WORDS; ++i) {
+        Piece<T> p;
+        p.q = w[i];
+        float2 f[V / 2];
+        unpack(p, f);
+#pragma unroll
+        for (int e = 0; e < V / 2; ++e) q[i * (V / 2) + e] = f[e];
+      }
+    } else {
+      const T* w = flat + g * (G * 32) + lane;
+#pragma unroll
+      for (int e = 0; e < G / 2; ++e) q[e] = make_float2(to_f(w[2 * e * 32]), to_f(w[(2 * e + 1) * 32]));
+    }
+#pragma unroll
+    for (int e = 0; e < G / 2; ++e) q[e] = mul2(q[e], both(sign));
+  };
+  const int per = (groups + split - 1) / split, g0 = min(groups, part * per), g1 = min(groups, g0 + per);
+  constexpr float kHuge = 3.402823466e38f;
+  float m[N];
+  int mg[N];
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    m[j] = -INFINITY;
+    mg[j] = 0;
+  }
+  for (int g = g0; g < g1; ++g) {
+    float2 q[G / 2];
+    group(g, q);
+    float x = -INFINITY;
+#pragma unroll
+    for (int e = 0; e < G / 2; ++e) x = fmaxf(x, fmaxf(q[e].x, q[e].y));      // (which leaves NaN out)
+    x = fminf(x, kHuge);
+    if (N == 1) {
+      if (x > m[0]) { m[0] = x; mg[0] = g; }
+    } else {
+#pragma unroll
+      for (int j = N - 1; j >= 0; --j) {
+        const bool in = x > m[j], above = j > 0 && x > m[j > 0 ? j - 1 : 0];
+        m[j] = in ? (above ? m[j > 0 ? j - 1 : 0] : x) : m[j];
+        mg[j] = in ? (above ? mg[j > 0 ? j - 1 : 0] : g) : mg[j];
+      }
+    }
+  }
+  float bound = m[N - 1], first = m[0];
+  if (split > 1) {      // the N-th largest of the warps' largest maxima, some two times N of them
+    const int told = min(N, max(1, 2 * N / split));
+    float* out = reinterpret_cast<float*>(shared);
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+      if (j < told) out[(warp * N + j) * 32 + lane] = m[j];
+    __syncthreads();
+    float b[N];
+#pragma unroll
+    for (int j = 0; j < N; ++j) b[j] = -INFINITY;
+    for (int w = warp - part; w < warp - part + split; ++w)
+      for (int j = 0; j < told; ++j) route_insert(b, out[(w * N + j) * 32 + lane]);
+    bound = b[N - 1];
+    first = b[0];
+    __syncthreads();
+  }
+  bound = fmaxf(bound, -kHuge);
+  // the scores of those groups that reach the bound, and of them the n best
+  float v[N];
+  int id[N];
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    v[j] = -INFINITY;
+    id[j] = -1;
+  }
+  const int list_stride = blockDim.y * 32;
+  unsigned short* list = reinterpret_cast<unsigned short*>(shared) + (warp * 32 + lane);
+  unsigned short* chosen = list + kRouteList * list_stride;
+  int have = 0, visits = 0;
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    chosen[j * list_stride] = (unsigned short)mg[j];
+    visits += m[j] >= bound;
+  }
+  const auto score = [&](int e) { return BY_ROW ? reinterpret_cast<const T*>(tile + (size_t)lane * stride)[e] : flat[e * 32 + lane]; };
+  for (int j = 0; j < visits; ++j) {
+    const int g = chosen[j * list_stride];
+    float2 q[G / 2];
+    group(g, q);
+#pragma unroll
+    for (int e = 0; e < G; ++e) {
+      list[have * list_stride] = (unsigned short)(g * G + e);
+      have += (e & 1 ? q[e / 2].y : q[e / 2].x) >= bound;
+    }
+    if (have > kRouteList - G - 1 || j == visits - 1) {
+      for (int i = 0; i < have; ++i) {
+        const int e = list[i * list_stride];
+        route_insert_tied(v, id, route_value(score(e), sign), e);
+      }
+      have = 0;
+    }
+  }
+  if (split > 1) {       // the tile's first warp joins the others' lists
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < N; ++j) shared[(warp * N + j) * 32 + lane] = make_float2(v[j], __int_as_float(id[j]));
+    __syncthreads();
+    if (part == 0)
+      for (int w = warp + 1; w < warp + split; ++w)
+        for (int j = 0; j < N; ++j) {
+          const float2 o = shared[(w * N + j) * 32 + lane];
+          if (!(o.x > -INFINITY)) break;
+          route_insert_tied(v, id, o.x, __float_as_int(o.y));
+        }
+  }
+  const float q0 = first > -INFINITY ? first : 0.f;
+  float sum = 0.f;
+  if (over_all) {
+    const float2 a2 = both(a * kLog2E), off = both(-q0);
+    float2 s2 = both(0.f);
+    if (q0 < kHuge) {
+#pragma unroll 2
+      for (int g = g0; g < g1; ++g) {
+        float2 q[G / 2];
+        group(g, q);
+#pragma unroll
+        for (int e = 0; e < G / 2; ++e) {
+          const float2 x = mul2(a2, add2(q[e], off));
+          s2 = add2(s2, make_float2(exp2_fast(fmaxf(x.x, -INFINITY)), exp2_fast(fmaxf(x.y, -INFINITY))));
+        }
+      }
+    } else {      // perhaps an infinite one, which counts as the largest finite number
+      for (int g = g0; g < g1; ++g) {
+        float2 q[G / 2];
+        group(g, q);
+#pragma unroll
+        for (int e = 0; e < G / 2; ++e)
+          s2 = add2(s2, make_float2(exp2_fast(a2.x * (fminf(fmaxf(q[e].x, -INFINITY), kHuge) - q0)),
+                                    exp2_fast(a2.x * (fminf(fmaxf(q[e].y, -INFINITY), kHuge) - q0))));
+      }
+    }
+    sum = s2.x + s2.y;
+    if (split > 1) {
+      __syncthreads();
+      reinterpret_cast<float*>(shared)[warp * 32 + lane] = sum;
+      __syncthreads();
+      if (part == 0)
+        for (int w = warp + 1; w < warp + split; ++w) sum += reinterpret_cast<float*>(shared)[w * 32 + lane];
+    }
+  }
+  if (part != 0 || lane >= here) return;
+  const long long t = row0 + lane;
+  float z[N];
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    z[j] = id[j] >= 0 ? expf(a * (v[j] - q0)) : 0.f;
+    if (!over_all && j < n) sum += z[j];
+  }
+#pragma unroll
+  for (int j = 0; j < N; ++j)
+    if (j < n) {
+      ids[t * n + j] = id[j];
+      weights[t * n + j] = id[j] >= 0 ? z[j] / sum : 0.f;
+    }
+  best[t] = sign * q0;
+  total[t] = sum;
 }
 
 // ---- the gradient ----------------------------------------------------------------------------------------------------------------------
@@ -426,18 +665,54 @@ route_grad_lane_kernel(const float* dweights, const T* s, long long rs, long lon
 
 // ---- launches --------------------------------------------------------------------------------------------------------------------------
 
+// f(N): the lists' length, n rounded up.  (Longer lists than 8 take more registers and code than a lane per row is worth.)
+constexpr int kRouteLaneMax = 8;
+template <typename F>
+int with_list(int n, F&& f) {
+  using std::integral_constant;
+  if (n == 1) return f(integral_constant<int, 1>());
+  if (n == 2) return f(integral_constant<int, 2>());
+  if (n <= 4) return f(integral_constant<int, 4>());
+  return f(integral_constant<int, 8>());
+}
+// Warps that share 32 rows: as many as it takes to fill the device (16 a processor), each with `least` scores of a row or more, and lists
+// that fit 32 KB together.
+inline int route_split(long long tiles, int k, int n, int least, int sms) {
+  int split = 1;
+  while (split < 16 && split * n < 128 && tiles * split < (long long)sms * 16 && k / split >= 2 * least) split *= 2;
+  return split;
+}
+
 template <typename T>
 int route_launch(const T* s, long long rs, long long cs, int rows, int k, int n, float scale, bool over_all, int* ids, float* weights,
                  float* best, float* total, int sms, cudaStream_t stream) {
+  const long long tiles = ((long long)rows + 31) / 32;
+  // 32 rows in shared memory, where they lie in whole words and fit
+  const bool by_row = cs == 1 && rows_aligned(s, rs, rows, k, sizeof(T));
+  const bool by_col = !by_row && rs == 1 && aligned(s, 16) && (cs * sizeof(T)) % 16 == 0;
+  const size_t bytes = RouteTile<T>::bytes(k, by_row);
+  if (n <= kRouteLaneMax && (by_row || by_col) && bytes <= kRouteTileBytes) {
+    // at least two warps for what 16 KB of scores keep waiting
+    int split = route_split(tiles, k, n, 32, sms);
+    while (split < 8 && split * n < 128 && bytes / split > (16 << 10)) split *= 2;
+    int per_cta = 1;
+    while (per_cta * split < 4 && bytes * per_cta * 2 <= kRouteTileBytes / 2 && tiles >= (long long)sms * 2 * per_cta) per_cta *= 2;
+    const int warps = per_cta * split;
+    return with_list(n, [&](auto count) -> int {
+      constexpr int N = count();
+      const size_t smem = bytes * per_cta + (size_t)32 * warps * std::max<size_t>((kRouteList + N) * 2, split > 1 ? N * 8 : 0);
+      const auto fn = by_row ? route_tile_kernel<T, N, true> : route_tile_kernel<T, N, false>;
+      KM_CUDA(allow_smem(fn, smem));
+      fn<<<(unsigned)((tiles + per_cta - 1) / per_cta), dim3(32, warps), smem, stream>>>(s, rs, cs, rows, k, n, scale, over_all, split,
+                                                                                       (int)bytes, ids, weights, best, total);
+      KM_CUDA(cudaGetLastError());
+      return KM_OK;
+    });
+  }
   // a lane per row where lanes' loads lie side by side, or a row is no longer than the line that its lane's loads share
-  if (cs != 1 || (size_t)k * sizeof(T) <= 128 || (rs == 1 && rows > 1)) {
-    const long long tiles = ((long long)rows + 31) / 32;
-    int most = 16;
-    while (most * n > 128) most /= 2;       // the lists that the warps of a tile exchange: 32 KB
-    int split = 1;
-    while (split < most && tiles * split < (long long)sms * 16 && k / split >= 64) split *= 2;
-    const int warps = std::max(4, split), per_cta = warps / split;
-    const auto launch = [&](auto count) -> int {
+  if (n <= kRouteLaneMax && (cs != 1 || (size_t)k * sizeof(T) <= 128 || (rs == 1 && rows > 1))) {
+    const int split = route_split(tiles, k, n, 64, sms), warps = std::max(4, split), per_cta = warps / split;
+    return with_list(n, [&](auto count) -> int {
       constexpr int N = count();
       const size_t smem = sizeof(float2) * 32 * warps * std::max(N == 1 ? 1 : kRouteList, split > 1 ? N : 1);
       const auto fn = route_lane_kernel<T, N>;
@@ -446,25 +721,21 @@ int route_launch(const T* s, long long rs, long long cs, int rows, int k, int n,
                                                                                        ids, weights, best, total);
       KM_CUDA(cudaGetLastError());
       return KM_OK;
-    };
-    using std::integral_constant;
-    if (n == 1) return launch(integral_constant<int, 1>());
-    if (n == 2) return launch(integral_constant<int, 2>());
-    if (n <= 4) return launch(integral_constant<int, 4>());
-    if (n <= 8) return launch(integral_constant<int, 8>());
-    if (n <= 16) return launch(integral_constant<int, 16>());
-    return launch(integral_constant<int, 32>());
+    });
   }
-  const bool al = rows_aligned(s, rs, rows, k, sizeof(T));
   const int pieces = (k + Piece<T>::V - 1) / Piece<T>::V;
-  const auto pick = [&](auto aligned_) {
-    constexpr bool AL = aligned_();
-    return pieces <= 32 ? route_warp_kernel<T, 1, AL> : pieces <= 64 ? route_warp_kernel<T, 2, AL>
-         : pieces <= 128 ? route_warp_kernel<T, 4, AL> : route_warp_kernel<T, 0, AL>;
+  const auto pick = [&](auto lie) {
+    constexpr RouteRows L = lie();
+    return pieces <= 32 ? route_warp_kernel<T, 1, L> : pieces <= 64 ? route_warp_kernel<T, 2, L>
+         : pieces <= 128 ? route_warp_kernel<T, 4, L> : route_warp_kernel<T, 0, L>;
   };
-  const auto fn = al ? pick(std::true_type()) : pick(std::false_type());
-  fn<<<(rows + kRouteWarps - 1) / kRouteWarps, kRouteWarps * 32, 0, stream>>>(s, rs, span_of<T>(s, rs, rows, k), rows, k, n, scale,
-                                                                            over_all, ids, weights, best, total);
+  using std::integral_constant;
+  auto fn = route_warp_kernel<T, 0, kStrided>;
+  if (cs == 1) fn = rows_aligned(s, rs, rows, k, sizeof(T)) ? pick(integral_constant<RouteRows, kAligned>())
+                                                            : pick(integral_constant<RouteRows, kUnaligned>());
+  fn<<<(rows + kRouteWarps - 1) / kRouteWarps, kRouteWarps * 32, 0, stream>>>(
+      s, rs, cs, cs == 1 ? span_of<T>(s, rs, rows, k) : Span<T>{nullptr, nullptr}, rows, k, n, scale, over_all, ids, weights, best,
+      total);
   KM_CUDA(cudaGetLastError());
   return KM_OK;
 }
