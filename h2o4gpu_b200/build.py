@@ -10,7 +10,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIBDIR = os.path.join(HERE, "lib")
 LIB = os.path.join(LIBDIR, "libh2o4gpu_kmeans.so")
-SOURCES = ["kmeans_api.cu", "kmeans_noalloc.cu", "kmeans_rows.cu"]
+SOURCES = ["kmeans_api.cu", "kmeans_noalloc.cu", "kmeans_rows.cu", "kmeans_route.cu"]
 
 
 def _nccl_include():
@@ -42,7 +42,7 @@ def build(force=False, verbose=False):
     os.makedirs(LIBDIR, exist_ok=True)
     nvcc = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
     cmd = [nvcc, "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
-           "-shared", "-Xcompiler", "-fPIC", "--expt-relaxed-constexpr",
+           "-shared", "-Xcompiler", "-fPIC", "--expt-relaxed-constexpr", "--threads=%d" % len(SOURCES),
            "-o", LIB] + _nccl_include() + [os.path.join(CSRC, s) for s in SOURCES] + ["-ldl"]
     if verbose:
         cmd.insert(1, "-Xptxas=-v")

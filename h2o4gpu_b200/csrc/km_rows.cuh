@@ -48,6 +48,9 @@ __device__ __forceinline__ float cta_sum(float v, float* red) {
 }
 
 // ---- host side ----------------------------------------------------------------
+constexpr size_t kMaxRows = 0x7fff0000ULL;   // a row or a place is an int, and a grid has room for a few CTAs more
+
+inline cudaStream_t as_stream(void* s) { return static_cast<cudaStream_t>(s); }
 inline int elem_size(int dtype) {
   switch (dtype) {
     case KM_DTYPE_F32: return 4;

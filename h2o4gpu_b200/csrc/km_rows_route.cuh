@@ -88,10 +88,46 @@ __device__ __forceinline__ void route_insert(float (&v)[N], float q) {
   }
 }
 
+// The outputs of row t from its list, best first; a lane's n values go out together where they fill whole words.
+template <int N>
+__device__ __forceinline__ void route_store(long long t, int n, const float (&v)[N], const int (&id)[N], float q0, float sum,
+                                            bool over_all, float a, float sign, int* ids, float* weights, float* best, float* total) {
+  float z[N];
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    z[j] = id[j] >= 0 ? expf(a * (v[j] - q0)) : 0.f;
+    if (!over_all && j < n) sum += z[j];
+  }
+#pragma unroll
+  for (int j = 0; j < N; ++j) z[j] = id[j] >= 0 ? z[j] / sum : 0.f;
+  int* it = ids + t * n;
+  float* wt = weights + t * n;
+  const bool whole = n == N && ((reinterpret_cast<uintptr_t>(ids) | reinterpret_cast<uintptr_t>(weights)) & (N >= 4 ? 15 : 4 * N - 1)) == 0;
+  if (N >= 4 && whole) {
+#pragma unroll
+    for (int j = 0; j + 3 < N; j += 4) {
+      *reinterpret_cast<int4*>(it + j) = make_int4(id[j], id[j + 1], id[j + 2], id[j + 3]);
+      *reinterpret_cast<float4*>(wt + j) = make_float4(z[j], z[j + 1], z[j + 2], z[j + 3]);
+    }
+  } else if (N == 2 && whole) {
+    *reinterpret_cast<int2*>(it) = make_int2(id[0], id[N - 1]);
+    *reinterpret_cast<float2*>(wt) = make_float2(z[0], z[N - 1]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+      if (j < n) {
+        it[j] = id[j];
+        wt[j] = z[j];
+      }
+  }
+  best[t] = sign * q0;
+  total[t] = sum;
+}
+
 template <typename T, int N>
 __global__ void __launch_bounds__(512)
-route_lane_kernel(const T* s, long long rs, long long cs, int rows, int k, int n, float scale, bool over_all, int split, int* ids,
-                  float* weights, float* best, float* total) {
+route_lane_kernel(const T* s, long long rs, long long cs, int rows, int k, int n, float scale, bool over_all, int split, int share,
+                  int* ids, float* weights, float* best, float* total) {
   extern __shared__ float2 shared[];       // the lanes' lists, then what the warps of a tile tell each other
   const int lane = threadIdx.x, warp = threadIdx.y, part = warp % split;
   const long long tile = (long long)blockIdx.x * (blockDim.y / split) + warp / split;
@@ -137,8 +173,15 @@ route_lane_kernel(const T* s, long long rs, long long cs, int rows, int k, int n
     float m[N], g = -INFINITY;
 #pragma unroll
     for (int j = 0; j < N; ++j) m[j] = -INFINITY;
-    walk([&](T r, int) { g = fmaxf(g, sign * to_f(r)); },      // (which leaves NaN out)
-         [&] { route_insert(m, fminf(g, 3.402823466e38f)); g = -INFINITY; });
+    const auto end_group = [&] {
+      route_insert(m, fminf(g, 3.402823466e38f));
+      g = -INFINITY;
+    };
+    walk([&](T r, int e) {
+           g = fmaxf(g, sign * to_f(r));      // (which leaves NaN out)
+           if ((e + 1) % share == 0 && share < kRouteGroup) end_group();
+         },
+         [&] { end_group(); });
     if (split > 1) {      // the bound of all the row's groups
       float* told = reinterpret_cast<float*>(shared);
 #pragma unroll
@@ -198,20 +241,7 @@ route_lane_kernel(const T* s, long long rs, long long cs, int rows, int k, int n
     }
   }
   if (part != 0 || !valid) return;
-  float z[N];
-#pragma unroll
-  for (int j = 0; j < N; ++j) {
-    z[j] = id[j] >= 0 ? expf(a * (v[j] - q0)) : 0.f;
-    if (!over_all && j < n) sum += z[j];
-  }
-#pragma unroll
-  for (int j = 0; j < N; ++j)
-    if (j < n) {
-      ids[(long long)t * n + j] = id[j];
-      weights[(long long)t * n + j] = id[j] >= 0 ? z[j] / sum : 0.f;
-    }
-  best[t] = sign * q0;
-  total[t] = sum;
+  route_store<N>(t, n, v, id, q0, sum, over_all, a, sign, ids, weights, best, total);
 }
 
 // ---- one warp per row: scores that lie row after row ---------------------------------------------------------------------------------
@@ -220,7 +250,7 @@ constexpr int kRouteWarps = 8;
 
 enum RouteRows { kAligned, kUnaligned, kStrided };
 template <typename T, int HELD, RouteRows LIE>
-__global__ void __launch_bounds__(kRouteWarps * 32)
+__global__ void __launch_bounds__(kRouteWarps * 32, 4)
 route_warp_kernel(const T* s, long long rs, long long cs, Span<T> in, int rows, int k, int n, float scale, bool over_all, int* ids, float* weights,
                   float* best, float* total) {
   constexpr int V = Piece<T>::V;
@@ -285,14 +315,15 @@ route_warp_kernel(const T* s, long long rs, long long cs, Span<T> in, int rows, 
   // Only lanes whose maximum reaches the bound have scores that do: n of them, but for ties.  The warp looks through one such lane's
   // scores after the other (they come from L1).
   int have = 0;
+  const int u_end = per_lane * V;
   for (unsigned int lanes = __ballot_sync(0xffffffffu, own >= max(nth, 1u)); lanes; lanes &= lanes - 1) {
-    const int l = __ffs(lanes) - 1;
-    for (int u0 = 0; u0 < per_lane * V; u0 += 32) {
-      const int u = u0 + lane, e = (l + u / V * 32) * V + u % V;
-      const float q = u < per_lane * V && e < k ? sign * to_f(sr[LIE == kStrided ? e * cs : e]) : -INFINITY;
+    const int base = (__ffs(lanes) - 1) * V + lane / V * (32 * V) + lane % V;
+    for (int u = 0; u < u_end; u += 32) {
+      const int e = base + u * 32;
+      const float q = u + lane < u_end && e < k ? sign * to_f(sr[LIE == kStrided ? e * cs : e]) : -INFINITY;
       const unsigned int reach = __ballot_sync(0xffffffffu, q >= bound);
       const int at = have + __popc(reach & ((1u << lane) - 1u));
-      if (q >= bound && at < 32) list[at] = route_key(q, e);
+      if (q >= bound && at < 32) list[at] = ((unsigned long long)__float_as_uint(q) << 32) | (unsigned int)e;
       have += __popc(reach);
     }
   }
@@ -300,23 +331,31 @@ route_warp_kernel(const T* s, long long rs, long long cs, Span<T> in, int rows, 
   if (over_all) {
     const float2 a2 = both(a * kLog2E), off = both(-q0);
     float2 s2 = both(0.f);
-    const bool huge = q0 == 3.402823466e38f;      // perhaps an infinite one, which counts as this
-    walk([&](float2 (&q)[V / 2], int) {
+    if (q0 < 3.402823466e38f) {
+      walk([&](const float2 (&q)[V / 2], int) {
 #pragma unroll
-      for (int e = 0; e < V / 2; ++e) {
-        if (huge) q[e] = make_float2(fminf(fmaxf(q[e].x, -INFINITY), q0), fminf(fmaxf(q[e].y, -INFINITY), q0));
-        const float2 x = mul2(a2, add2(q[e], off));
-        s2 = add2(s2, make_float2(exp2_fast(fmaxf(x.x, -INFINITY)), exp2_fast(fmaxf(x.y, -INFINITY))));
-      }
-    });
-    sum = s2.x + s2.y;
+        for (int e = 0; e < V / 2; ++e) {
+          const float2 x = mul2(a2, add2(q[e], off));
+          s2 = add2(s2, make_float2(exp2_fast(fmaxf(x.x, -INFINITY)), exp2_fast(fmaxf(x.y, -INFINITY))));
+        }
+      });
+      sum = s2.x + s2.y;
+    } else {      // perhaps an infinite one, which counts as the largest finite number
+      for (int e = lane; e < k; e += 32) sum += exp2_fast(a2.x * (route_value(sr[LIE == kStrided ? e * cs : e], sign) - q0));
+    }
   }
   __syncwarp();
   // `mine`: this lane's score among the n best, `place` where it goes; lanes without one fill the places behind
   unsigned long long mine = 0ULL;
   int place = 0;
   if (have <= 32) {
-    mine = lane < have ? list[lane] : 0ULL;
+    if (lane < have) {
+      mine = list[lane];
+      mine = route_key(__uint_as_float((unsigned int)(mine >> 32)), (int)(unsigned int)mine);
+    }
+    __syncwarp();
+    list[lane] = mine;
+    __syncwarp();
     for (int i = 0; i < have; ++i) place += list[i] > mine;
     if (lane >= have) place = lane;
     if (place >= n) mine = 0ULL;
@@ -349,12 +388,15 @@ route_warp_kernel(const T* s, long long rs, long long cs, Span<T> in, int rows, 
 }
 
 // ---- one lane per row, the scores of 32 rows in shared memory --------------------------------------------------------------------------
-// What a row costs besides its scores is then paid once for 32 rows, and a lane can go back to the few groups that hold its n best - the n
-// with the largest maxima, ties to the lower: any other score comes behind n of those maxima.  `split` warps share a tile, each a
-// run of its groups; the warps then tell each other a bound and join their lists.
+// What a row costs besides its scores is then paid once for 32 rows.  `split` warps share a tile, each a run of its groups; the warps then
+// tell each other a bound and join their lists.
 //   BY_ROW: row r at r * stride bytes (an odd number of 16-byte words: lanes read those without bank conflicts); a group is 8 scores of it
 //   else:   cluster e's 32 scores at e * 32
 constexpr size_t kRouteTileBytes = 100 << 10;      // two CTAs a processor
+// Rows of some 1 KB: a warp per row costs the same whatever the row's length up to 2 KB, a lane per row grows with it.  8 of 256 float32 of
+// 65,536 rows 37 us with a lane per row and 63 with a warp, of 512 bfloat16 47 and 66, of 512 float32 78 and 71, of 1000 bfloat16 (32,768
+// rows) 50 and 41.
+constexpr size_t kRouteRowTileBytes = 40 << 10;
 template <typename T>
 struct RouteTile {
   static constexpr int G = kRouteGroup, WORDS = G * (int)sizeof(T) / 16;      // 16-byte words of a group
@@ -363,25 +405,10 @@ struct RouteTile {
   static size_t bytes(int k, bool by_row) { return by_row ? (size_t)32 * stride(k) : (size_t)groups(k) * G * 32 * sizeof(T); }
 };
 
-// Into a list of N sorted by descending quality, ties by cluster.
-template <int N>
-__device__ __forceinline__ void route_insert_tied(float (&v)[N], int (&id)[N], float q, int e) {
-  const auto before = [&](int j) { return q > v[j] || (q == v[j] && e < id[j]); };
-  if (!before(N - 1)) return;
-#pragma unroll
-  for (int j = N - 1; j >= 0; --j) {
-    const bool here = before(j), above = j > 0 && before(j > 0 ? j - 1 : 0);
-    if (here) {
-      v[j] = above ? v[j > 0 ? j - 1 : 0] : q;
-      id[j] = above ? id[j > 0 ? j - 1 : 0] : e;
-    }
-  }
-}
-
 template <typename T, int N, bool BY_ROW>
 __global__ void __launch_bounds__(512)
-route_tile_kernel(const T* s, long long rs, long long cs, int rows, int k, int n, float scale, bool over_all, int split, int tile_bytes,
-                  int* ids, float* weights, float* best, float* total) {
+route_tile_kernel(const T* s, long long rs, long long cs, int rows, int k, int n, float scale, bool over_all, int split, int share,
+                  int tile_bytes, int* ids, float* weights, float* best, float* total) {
   using Tile = RouteTile<T>;
   constexpr int G = Tile::G, WORDS = Tile::WORDS, V = Piece<T>::V;
   extern __shared__ uint4 tiles[];
@@ -442,28 +469,30 @@ route_tile_kernel(const T* s, long long rs, long long cs, int rows, int k, int n
   const int per = (groups + split - 1) / split, g0 = min(groups, part * per), g1 = min(groups, g0 + per);
   constexpr float kHuge = 3.402823466e38f;
   float m[N];
-  int mg[N];
 #pragma unroll
-  for (int j = 0; j < N; ++j) {
-    m[j] = -INFINITY;
-    mg[j] = 0;
-  }
+  for (int j = 0; j < N; ++j) m[j] = -INFINITY;
   for (int g = g0; g < g1; ++g) {
     float2 q[G / 2];
     group(g, q);
-    float x = -INFINITY;
+    if (share == 1) {
 #pragma unroll
-    for (int e = 0; e < G / 2; ++e) x = fmaxf(x, fmaxf(q[e].x, q[e].y));      // (which leaves NaN out)
-    x = fminf(x, kHuge);
-    if (N == 1) {
-      if (x > m[0]) { m[0] = x; mg[0] = g; }
-    } else {
-#pragma unroll
-      for (int j = N - 1; j >= 0; --j) {
-        const bool in = x > m[j], above = j > 0 && x > m[j > 0 ? j - 1 : 0];
-        m[j] = in ? (above ? m[j > 0 ? j - 1 : 0] : x) : m[j];
-        mg[j] = in ? (above ? mg[j > 0 ? j - 1 : 0] : g) : mg[j];
+      for (int e = 0; e < G / 2; ++e) {
+        route_insert(m, fminf(fmaxf(q[e].x, -INFINITY), kHuge));
+        route_insert(m, fminf(fmaxf(q[e].y, -INFINITY), kHuge));
       }
+      continue;
+    }
+    float x[G / 2];
+#pragma unroll
+    for (int e = 0; e < G / 2; ++e) x[e] = fminf(fmaxf(fmaxf(q[e].x, q[e].y), -INFINITY), kHuge);      // (which leaves NaN out)
+    if (share == 2) {
+#pragma unroll
+      for (int e = 0; e < G / 2; ++e) route_insert(m, x[e]);
+    } else if (share == 4) {
+      route_insert(m, fmaxf(x[0], x[1]));
+      route_insert(m, fmaxf(x[2], x[3]));
+    } else {
+      route_insert(m, fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])));
     }
   }
   float bound = m[N - 1], first = m[0];
@@ -484,7 +513,7 @@ route_tile_kernel(const T* s, long long rs, long long cs, int rows, int k, int n
     __syncthreads();
   }
   bound = fmaxf(bound, -kHuge);
-  // the scores of those groups that reach the bound, and of them the n best
+  // the scores that reach the bound, in the clusters' order, and of them the n best
   float v[N];
   int id[N];
 #pragma unroll
@@ -493,32 +522,40 @@ route_tile_kernel(const T* s, long long rs, long long cs, int rows, int k, int n
     id[j] = -1;
   }
   const int list_stride = blockDim.y * 32;
-  unsigned short* list = reinterpret_cast<unsigned short*>(shared) + (warp * 32 + lane);
-  unsigned short* chosen = list + kRouteList * list_stride;
-  int have = 0, visits = 0;
-#pragma unroll
-  for (int j = 0; j < N; ++j) {
-    chosen[j * list_stride] = (unsigned short)mg[j];
-    visits += m[j] >= bound;
-  }
-  const auto score = [&](int e) { return BY_ROW ? reinterpret_cast<const T*>(tile + (size_t)lane * stride)[e] : flat[e * 32 + lane]; };
-  for (int j = 0; j < visits; ++j) {
-    const int g = chosen[j * list_stride];
+  unsigned short* const list = reinterpret_cast<unsigned short*>(shared) + (warp * 32 + lane);
+  unsigned short* end = list;
+  const auto put = [&] {
+    for (const unsigned short* i = list; i != end; i += list_stride) {
+      const int e = *i;
+      route_insert(v, id, route_value(BY_ROW ? reinterpret_cast<const T*>(tile + (size_t)lane * stride)[e] : flat[e * 32 + lane], sign),
+                   e);
+    }
+    end = list;
+  };
+  const float q0 = first > -INFINITY ? first : 0.f;
+  const float2 a2 = both(a * kLog2E), off = both(-q0);
+  float2 s2 = both(0.f);
+  for (int g = g0; g < g1; ++g) {
     float2 q[G / 2];
     group(g, q);
 #pragma unroll
     for (int e = 0; e < G; ++e) {
-      list[have * list_stride] = (unsigned short)(g * G + e);
-      have += (e & 1 ? q[e / 2].y : q[e / 2].x) >= bound;
+      *end = (unsigned short)(g * G + e);      // kept if the next one does not overwrite it
+      if ((e & 1 ? q[e / 2].y : q[e / 2].x) >= bound) end += list_stride;
     }
-    if (have > kRouteList - G - 1 || j == visits - 1) {
-      for (int i = 0; i < have; ++i) {
-        const int e = list[i * list_stride];
-        route_insert_tied(v, id, route_value(score(e), sign), e);
+    if (end > list + (kRouteList - G - 1) * list_stride) put();
+    if (over_all) {
+      if (q0 == kHuge)      // perhaps an infinite score, which counts as this
+#pragma unroll
+        for (int e = 0; e < G / 2; ++e) q[e] = make_float2(fminf(fmaxf(q[e].x, -INFINITY), kHuge), fminf(fmaxf(q[e].y, -INFINITY), kHuge));
+#pragma unroll
+      for (int e = 0; e < G / 2; ++e) {
+        const float2 x = mul2(a2, add2(q[e], off));
+        s2 = add2(s2, make_float2(exp2_fast(fmaxf(x.x, -INFINITY)), exp2_fast(fmaxf(x.y, -INFINITY))));
       }
-      have = 0;
     }
   }
+  put();
   if (split > 1) {       // the tile's first warp joins the others' lists
     __syncthreads();
 #pragma unroll
@@ -529,35 +566,11 @@ route_tile_kernel(const T* s, long long rs, long long cs, int rows, int k, int n
         for (int j = 0; j < N; ++j) {
           const float2 o = shared[(w * N + j) * 32 + lane];
           if (!(o.x > -INFINITY)) break;
-          route_insert_tied(v, id, o.x, __float_as_int(o.y));
+          route_insert(v, id, o.x, __float_as_int(o.y));
         }
   }
-  const float q0 = first > -INFINITY ? first : 0.f;
   float sum = 0.f;
   if (over_all) {
-    const float2 a2 = both(a * kLog2E), off = both(-q0);
-    float2 s2 = both(0.f);
-    if (q0 < kHuge) {
-#pragma unroll 2
-      for (int g = g0; g < g1; ++g) {
-        float2 q[G / 2];
-        group(g, q);
-#pragma unroll
-        for (int e = 0; e < G / 2; ++e) {
-          const float2 x = mul2(a2, add2(q[e], off));
-          s2 = add2(s2, make_float2(exp2_fast(fmaxf(x.x, -INFINITY)), exp2_fast(fmaxf(x.y, -INFINITY))));
-        }
-      }
-    } else {      // perhaps an infinite one, which counts as the largest finite number
-      for (int g = g0; g < g1; ++g) {
-        float2 q[G / 2];
-        group(g, q);
-#pragma unroll
-        for (int e = 0; e < G / 2; ++e)
-          s2 = add2(s2, make_float2(exp2_fast(a2.x * (fminf(fmaxf(q[e].x, -INFINITY), kHuge) - q0)),
-                                    exp2_fast(a2.x * (fminf(fmaxf(q[e].y, -INFINITY), kHuge) - q0))));
-      }
-    }
     sum = s2.x + s2.y;
     if (split > 1) {
       __syncthreads();
@@ -569,20 +582,7 @@ route_tile_kernel(const T* s, long long rs, long long cs, int rows, int k, int n
   }
   if (part != 0 || lane >= here) return;
   const long long t = row0 + lane;
-  float z[N];
-#pragma unroll
-  for (int j = 0; j < N; ++j) {
-    z[j] = id[j] >= 0 ? expf(a * (v[j] - q0)) : 0.f;
-    if (!over_all && j < n) sum += z[j];
-  }
-#pragma unroll
-  for (int j = 0; j < N; ++j)
-    if (j < n) {
-      ids[t * n + j] = id[j];
-      weights[t * n + j] = id[j] >= 0 ? z[j] / sum : 0.f;
-    }
-  best[t] = sign * q0;
-  total[t] = sum;
+  route_store<N>(t, n, v, id, q0, sum, over_all, a, sign, ids, weights, best, total);
 }
 
 // ---- the gradient ----------------------------------------------------------------------------------------------------------------------
@@ -675,6 +675,12 @@ int with_list(int n, F&& f) {
   if (n <= 4) return f(integral_constant<int, 4>());
   return f(integral_constant<int, 8>());
 }
+// Scores whose maximum stands for them in the first walk: so many that four times N groups remain, and the bound lets few others pass.
+inline int route_share(int k, int n) {
+  int share = kRouteGroup;
+  while (share > 1 && k / share < 4 * n) share /= 2;
+  return share;
+}
 // Warps that share 32 rows: as many as it takes to fill the device (16 a processor), each with `least` scores of a row or more, and lists
 // that fit 32 KB together.
 inline int route_split(long long tiles, int k, int n, int least, int sms) {
@@ -689,9 +695,10 @@ int route_launch(const T* s, long long rs, long long cs, int rows, int k, int n,
   const long long tiles = ((long long)rows + 31) / 32;
   // 32 rows in shared memory, where they lie in whole words and fit
   const bool by_row = cs == 1 && rows_aligned(s, rs, rows, k, sizeof(T));
-  const bool by_col = !by_row && rs == 1 && aligned(s, 16) && (cs * sizeof(T)) % 16 == 0;
+  // (the best one of scores that lie cluster after cluster needs one walk, which is as fast from memory: 65,536 x 512 float32 33 us, 48 by tiles)
+  const bool by_col = !by_row && n > 1 && rs == 1 && aligned(s, 16) && (cs * sizeof(T)) % 16 == 0;
   const size_t bytes = RouteTile<T>::bytes(k, by_row);
-  if (n <= kRouteLaneMax && (by_row || by_col) && bytes <= kRouteTileBytes) {
+  if (n <= kRouteLaneMax && (by_row || by_col) && bytes <= (by_row ? kRouteRowTileBytes : kRouteTileBytes)) {
     // at least two warps for what 16 KB of scores keep waiting
     int split = route_split(tiles, k, n, 32, sms);
     while (split < 8 && split * n < 128 && bytes / split > (16 << 10)) split *= 2;
@@ -700,11 +707,12 @@ int route_launch(const T* s, long long rs, long long cs, int rows, int k, int n,
     const int warps = per_cta * split;
     return with_list(n, [&](auto count) -> int {
       constexpr int N = count();
-      const size_t smem = bytes * per_cta + (size_t)32 * warps * std::max<size_t>((kRouteList + N) * 2, split > 1 ? N * 8 : 0);
+      const size_t smem = bytes * per_cta + (size_t)32 * warps * std::max<size_t>(kRouteList * 2, split > 1 ? N * 8 : 0);
       const auto fn = by_row ? route_tile_kernel<T, N, true> : route_tile_kernel<T, N, false>;
       KM_CUDA(allow_smem(fn, smem));
       fn<<<(unsigned)((tiles + per_cta - 1) / per_cta), dim3(32, warps), smem, stream>>>(s, rs, cs, rows, k, n, scale, over_all, split,
-                                                                                       (int)bytes, ids, weights, best, total);
+                                                                                       route_share(k, N), (int)bytes, ids, weights,
+                                                                                       best, total);
       KM_CUDA(cudaGetLastError());
       return KM_OK;
     });
@@ -718,7 +726,7 @@ int route_launch(const T* s, long long rs, long long cs, int rows, int k, int n,
       const auto fn = route_lane_kernel<T, N>;
       KM_CUDA(allow_smem(fn, smem));
       fn<<<(unsigned)((tiles + per_cta - 1) / per_cta), dim3(32, warps), smem, stream>>>(s, rs, cs, rows, k, n, scale, over_all, split,
-                                                                                       ids, weights, best, total);
+                                                                                       route_share(k, N), ids, weights, best, total);
       KM_CUDA(cudaGetLastError());
       return KM_OK;
     });

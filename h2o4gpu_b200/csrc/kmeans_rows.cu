@@ -1,17 +1,13 @@
-// C entry points of the row operators (section 5 of include/h2o4gpu_kmeans.h): layer norm, routing to the nearest clusters,
-// rows sorted by cluster and back.  They work on device memory of the current device, enqueue on the caller's stream, never
-// allocate and never wait.
+// C entry points of the row operators (section 5 of include/h2o4gpu_kmeans.h): layer norm, rows sorted by cluster and back (routing:
+// kmeans_route.cu).  They work on device memory of the current device, enqueue on the caller's stream, never allocate and never wait.
 #include "km_rows_move.cuh"
 #include "km_rows_norm.cuh"
-#include "km_rows_route.cuh"
 #include "km_rows_sort.cuh"
 
 using namespace km;
 using namespace km::rows;
 
 namespace {
-
-constexpr size_t kMaxRows = 0x7fff0000ULL;   // a row or a place is an int, and a grid has room for a few CTAs more
 
 // Type of the norm's weight and bias: float32, or the rows' own.
 #define KM_ROWS_PARAM(param_dtype, T, P, ...)                       \
@@ -128,54 +124,6 @@ int layer_norm_grad(int dtype, const void* dy, long long dys, const void* x, lon
     KM_CUDA(cudaGetLastError());
   }
   return KM_OK;
-}
-
-// Scores lie in any two strides; a value's place must fit 63 bits.
-bool strides_ok(long long rs, long long cs) { return rs >= 0 && cs >= 0 && rs <= (1LL << 31) && cs <= (1LL << 31); }
-
-int check_route(const char* name, int dtype, size_t rows, int k, int n, float scale) {
-  if (!elem_size(dtype)) KM_FAIL(KM_EINVAL, std::string(name) + ": scores are float32, float16 or bfloat16");
-  if (rows > kMaxRows || k < 1 || k > kRouteMaxK) KM_FAIL(KM_EINVAL, std::string(name) + ": bad argument");
-  if (n < 1 || n > kRouteMax || n > k)
-    KM_FAIL(KM_EINVAL, std::string(name) + ": a row takes 1 to " + std::to_string(kRouteMax) + " clusters, and no more than there are");
-  if (!std::isfinite(scale) || scale == 0.f) KM_FAIL(KM_EINVAL, std::string(name) + ": scale must be finite and not zero");
-  return KM_OK;
-}
-
-int route(int dtype, const void* scores, long long rs, long long cs, size_t rows, int k, int n, float scale, int over_all,
-          int32_t* ids, float* weights, float* best, float* total, cudaStream_t stream) {
-  KM_TRY(check_route("kmeans_route", dtype, rows, k, n, scale));
-  if (rows == 0) return KM_OK;
-  if (!scores || !aligned(scores, elem_size(dtype)) || !strides_ok(rs, cs) || !ids || !weights || !best || !total ||
-      !aligned(ids, 4) || !aligned(weights, 4) || !aligned(best, 4) || !aligned(total, 4))
-    KM_FAIL(KM_EINVAL, "kmeans_route: bad argument");
-  int sms = 0, rc = KM_OK;
-  KM_TRY(sm_count(&sms));
-  KM_ROWS_DTYPE(dtype, T,
-      rc = route_launch<T>(static_cast<const T*>(scores), rs, cs, (int)rows, k, n, scale, over_all != 0, ids, weights, best, total, sms,
-                           stream));
-  return rc;
-}
-
-int route_grad(int dtype, const float* dweights, const void* scores, long long rs, long long cs, size_t rows, int k, int n,
-               float scale, int over_all, const int32_t* ids, const float* weights, const float* best, const float* total,
-               void* dscores, long long drs, long long dcs, cudaStream_t stream) {
-  KM_TRY(check_route("kmeans_route_grad", dtype, rows, k, n, scale));
-  if (rows == 0) return KM_OK;
-  const int size = elem_size(dtype);
-  if (!dweights || !ids || !weights || !aligned(dweights, 4) || !aligned(ids, 4) || !aligned(weights, 4) || !dscores ||
-      !aligned(dscores, size) || !strides_ok(drs, dcs))
-    KM_FAIL(KM_EINVAL, "kmeans_route_grad: bad argument");
-  if (over_all && (!scores || !aligned(scores, size) || !strides_ok(rs, cs) || !best || !total || !aligned(best, 4) || !aligned(total, 4)))
-    KM_FAIL(KM_EINVAL, "kmeans_route_grad: weights over all clusters need the scores, best and total");
-  if (!((dcs == 1 && (drs >= k || rows == 1)) || (drs == 1 && (dcs >= (long long)rows || k == 1))))
-    KM_FAIL(KM_EINVAL, "kmeans_route_grad: dscores must lie row after row or cluster after cluster");
-  int sms = 0, rc = KM_OK;
-  KM_TRY(sm_count(&sms));
-  KM_ROWS_DTYPE(dtype, T,
-      rc = route_grad_launch<T>(dweights, static_cast<const T*>(scores), rs, cs, (int)rows, k, n, scale, over_all != 0, ids, weights,
-                                best, total, static_cast<T*>(dscores), drs, dcs, sms, stream));
-  return rc;
 }
 
 int check_sort(const char* name, size_t rows, int n, int k, int align, size_t* capacity) {
@@ -323,8 +271,6 @@ int combine_grad(int dtype, const void* dy, long long dys, const void* in, long 
   return KM_OK;
 }
 
-cudaStream_t as_stream(void* s) { return static_cast<cudaStream_t>(s); }
-
 }  // namespace
 
 extern "C" {
@@ -344,20 +290,6 @@ int kmeans_layer_norm_grad(int dtype, const void* dy, long long dy_stride, const
   return guarded("kmeans_layer_norm_grad", [&] {
     return layer_norm_grad(dtype, dy, dy_stride, x, x_stride, mean, rstd, rows, cols, weight, param_dtype, dx, dx_stride, dweight,
                            dbias, workspace, workspace_bytes, as_stream(stream));
-  });
-}
-int kmeans_route(int dtype, const void* scores, long long row_stride, long long col_stride, size_t rows, int k, int n, float scale,
-                 int over_all, int32_t* ids, float* weights, float* best, float* total, void* stream) {
-  return guarded("kmeans_route", [&] {
-    return route(dtype, scores, row_stride, col_stride, rows, k, n, scale, over_all, ids, weights, best, total, as_stream(stream));
-  });
-}
-int kmeans_route_grad(int dtype, const float* dweights, const void* scores, long long row_stride, long long col_stride, size_t rows,
-                      int k, int n, float scale, int over_all, const int32_t* ids, const float* weights, const float* best,
-                      const float* total, void* dscores, long long drow_stride, long long dcol_stride, void* stream) {
-  return guarded("kmeans_route_grad", [&] {
-    return route_grad(dtype, dweights, scores, row_stride, col_stride, rows, k, n, scale, over_all, ids, weights, best, total, dscores,
-                      drow_stride, dcol_stride, as_stream(stream));
   });
 }
 int kmeans_sort_rows_sizes(size_t rows, int n, int k, int align, size_t* capacity, size_t* workspace_bytes) {
