@@ -699,9 +699,10 @@ int route_launch(const T* s, long long rs, long long cs, int rows, int k, int n,
   const bool by_col = !by_row && n > 1 && rs == 1 && aligned(s, 16) && (cs * sizeof(T)) % 16 == 0;
   const size_t bytes = RouteTile<T>::bytes(k, by_row);
   if (n <= kRouteLaneMax && (by_row || by_col) && bytes <= (by_row ? kRouteRowTileBytes : kRouteTileBytes)) {
-    // at least two warps for what 16 KB of scores keep waiting
+    // more warps for a tile than its rows fill, so that the tiles a processor holds keep it busy (what the warps tell each other costs more
+    // for longer lists)
     int split = route_split(tiles, k, n, 32, sms);
-    while (split < 8 && split * n < 128 && bytes / split > (16 << 10)) split *= 2;
+    while (split < 8 && split * n < 128 && bytes / split > (size_t)((n <= 4 ? 8 : 16) << 10)) split *= 2;
     int per_cta = 1;
     while (per_cta * split < 4 && bytes * per_cta * 2 <= kRouteTileBytes / 2 && tiles >= (long long)sms * 2 * per_cta) per_cta *= 2;
     const int warps = per_cta * split;

@@ -16,33 +16,35 @@ constexpr size_t kSortTables = 196608;    // bytes of those tables
 // How one call is cut: `blocks` CTAs of `chunk` entries each, in order; `warps` warps of a CTA keep counts of their own.
 struct SortPlan {
   int blocks = 1, warps = 1;
-  long long chunk = 0;
+  int chunk = 0;
 };
 inline SortPlan sort_plan(long long entries, int k, int sms) {
   SortPlan p;
-  // One CTA, one launch, while counting on a second one would cost more than it saves; else as many as there are
-  // processors, each with enough entries that reading the others' counts (blocks x k words) stays small beside them.
-  const long long per = std::max<long long>(4096, k);
-  p.blocks = (int)std::min<long long>(sms, std::max<long long>(1, entries / per));
-  p.chunk = (entries + p.blocks - 1) / p.blocks;
+  // One CTA, one launch, up to 2048 entries.  Else as many as there are processors, with two entries a thread or more, and so few that what
+  // all of them read of each other's counts (blocks^2 x k words, from L2) stays below 64 MB.
+  long long most = std::min<long long>(sms, entries / (2 * kSortThreads));
+  while (most > 1 && most * most * k > (16 << 20)) --most;
+  p.blocks = (int)std::max<long long>(1, most);
+  p.chunk = (int)((entries + p.blocks - 1) / p.blocks);
   p.warps = kSortThreads / 32;
-  while (p.warps > 1 && (size_t)(p.warps + 1) * k * 4 > kSortTables) p.warps /= 2;
+  while (p.warps > 1 && (size_t)(p.warps + 2) * k * 4 > kSortTables) p.warps /= 2;
   return p;
 }
 
-__device__ __forceinline__ int sort_id(const int* ids, long long stride, int n, long long i, int k) {
-  const int id = ids[n == 1 ? i * stride : (i / n) * stride + i % n];
+// Entry i's cluster; entries lie side by side (stride n) but for strided ids.
+__device__ __forceinline__ int sort_id(const int* ids, long long stride, int n, int i, int k) {
+  const int id = ids[stride == n ? (long long)i : (i / n) * stride + i % n];
   return id >= 0 && id < k ? id : -1;
 }
 
 // Entries of each cluster in every chunk: part[block * k + cluster].
 __global__ void __launch_bounds__(kSortThreads)
-sort_count_kernel(const int* ids, long long stride, int n, long long entries, int k, long long chunk, int* part) {
+sort_count_kernel(const int* ids, long long stride, int n, int entries, int k, int chunk, int* part) {
   extern __shared__ int hist[];
   for (int e = threadIdx.x; e < k; e += kSortThreads) hist[e] = 0;
   __syncthreads();
-  const long long i1 = min(entries, (blockIdx.x + 1) * chunk);
-  for (long long i = blockIdx.x * chunk + threadIdx.x; i < i1; i += kSortThreads) {
+  const int i0 = blockIdx.x * chunk, i1 = min((long long)entries, (long long)i0 + chunk);
+  for (int i = i0 + threadIdx.x; i < i1; i += kSortThreads) {
     const int id = sort_id(ids, stride, n, i, k);
     if (id >= 0) atomicAdd(&hist[id], 1);
   }
@@ -80,36 +82,45 @@ __device__ __forceinline__ int cta_scan(int v, int* red, int* total) {
 // Places of one chunk's entries.  Integer counts only: the order of the shared-memory additions does not matter, and the
 // ranks inside a warp come from the lanes' order.
 __global__ void __launch_bounds__(kSortThreads)
-sort_place_kernel(const int* ids, long long stride, int n, long long entries, int k, int align, SortPlan plan, const int* part,
-                  int* offsets, int* counts, int* slot, int* source, long long capacity) {
+sort_place_kernel(const int* ids, long long stride, int n, int entries, int k, int align, SortPlan plan, const int* part,
+                  int* offsets, int* counts, int* slot, int* source, int capacity) {
   extern __shared__ int tables[];
   __shared__ int red[32];
-  int* wcnt = tables;                       // [warps][k]: entries of each cluster per warp, then the next place
-  int* start = tables + (size_t)plan.warps * k;   // [k]: where the group starts
+  int* wcnt = tables;                                 // [warps][k]: entries of each cluster per warp, then the next place
+  int* sum = tables + (size_t)plan.warps * k;         // [k]: entries of each cluster
+  int* earlier = sum + k;                             // [k]: of those, in the chunks before this one
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, b = blockIdx.x;
-  for (int i = threadIdx.x; i < plan.warps * k; i += kSortThreads) wcnt[i] = 0;
+  for (int i = threadIdx.x; i < (plan.warps + 2) * k; i += kSortThreads) tables[i] = 0;
   __syncthreads();
-  const long long c0 = b * plan.chunk, c1 = min(entries, c0 + plan.chunk);
-  const long long per = (plan.chunk + plan.warps - 1) / plan.warps;
-  const long long w0 = min(c1, c0 + warp * per), w1 = min(c1, w0 + per);
+  const int c0 = b * plan.chunk, c1 = (int)min((long long)entries, (long long)c0 + plan.chunk);
+  const int per = ((plan.chunk + plan.warps - 1) / plan.warps + 31) / 32 * 32;
+  const int w0 = (int)min((long long)c1, (long long)c0 + (long long)warp * per), w1 = (int)min((long long)c1, (long long)w0 + per);
   if (warp < plan.warps)
-    for (long long i = w0 + lane; i < w1; i += 32) {
+    for (int i = w0 + lane; i < w1; i += 32) {
       const int id = sort_id(ids, stride, n, i, k);
       if (id >= 0) atomicAdd(&wcnt[(size_t)warp * k + id], 1);
     }
+  // every CTA adds up all chunks' counts, so that nothing has to wait for another CTA
+  if (part) {
+    const int words = plan.blocks * k, before = b * k;
+#pragma unroll 4
+    for (int i = threadIdx.x; i < words; i += kSortThreads) {
+      const int v = part[i], e = i % k;
+      if (v) {
+        atomicAdd(&sum[e], v);
+        if (i < before) atomicAdd(&earlier[e], v);
+      }
+    }
+  }
   __syncthreads();
-  // group starts: every CTA adds up all chunks' counts, so that nothing has to wait for another CTA
   int base = 0;
   for (int e0 = 0; e0 < k; e0 += kSortThreads) {
     const int e = e0 + threadIdx.x;
     int all = 0, before = 0;
     if (e < k) {
       if (part) {
-        for (int c = 0; c < plan.blocks; ++c) {
-          const int v = part[(size_t)c * k + e];
-          all += v;
-          if (c < b) before += v;
-        }
+        all = sum[e];
+        before = earlier[e];
       } else {
         for (int w = 0; w < plan.warps; ++w) all += wcnt[(size_t)w * k + e];
       }
@@ -118,7 +129,6 @@ sort_place_kernel(const int* ids, long long stride, int n, long long entries, in
     int total;
     const int at = base + cta_scan(e < k ? padded : 0, red, &total);
     if (e < k) {
-      start[e] = at;
       if (b == 0) {
         offsets[e] = at;
         counts[e] = all;
@@ -136,12 +146,11 @@ sort_place_kernel(const int* ids, long long stride, int n, long long entries, in
     base += total;
   }
   if (b == 0 && threadIdx.x == 0) offsets[k] = base;
-  for (long long p = base + (long long)b * kSortThreads + threadIdx.x; p < capacity; p += (long long)plan.blocks * kSortThreads)
-    source[p] = -1;
+  for (long long p = base + (long long)b * kSortThreads + threadIdx.x; p < capacity; p += plan.blocks * kSortThreads) source[p] = -1;
   __syncthreads();
   if (warp < plan.warps)
-    for (long long i0 = w0; i0 < w1; i0 += 32) {
-      const long long i = i0 + lane;
+    for (int i0 = w0; i0 < w1; i0 += 32) {
+      const int i = i0 + lane;
       const int id = i < w1 ? sort_id(ids, stride, n, i, k) : -1;
       const unsigned int same = __match_any_sync(0xffffffffu, id);
       int place = -1;
@@ -151,7 +160,7 @@ sort_place_kernel(const int* ids, long long stride, int n, long long entries, in
       __syncwarp();
       if (i < w1) {
         slot[i] = place;
-        if (place >= 0) source[place] = (int)i;
+        if (place >= 0) source[place] = i;
       }
     }
 }

@@ -162,7 +162,7 @@ int sort_rows(const int32_t* ids, long long stride, size_t rows, int n, int k, i
     KM_FAIL(KM_EINVAL, "kmeans_sort_rows: bad argument");
   int sms = 0;
   KM_TRY(sm_count(&sms));
-  const long long entries = (long long)rows * n;
+  const int entries = (int)(rows * (size_t)n);
   const SortPlan plan = sort_plan(entries, k, sms);
   int* part = nullptr;
   if (plan.blocks > 1) {
@@ -174,10 +174,10 @@ int sort_rows(const int32_t* ids, long long stride, size_t rows, int n, int k, i
     sort_count_kernel<<<plan.blocks, kSortThreads, smem, stream>>>(ids, stride, n, entries, k, plan.chunk, part);
     KM_CUDA(cudaGetLastError());
   }
-  const size_t smem = (size_t)(plan.warps + 1) * k * sizeof(int);
+  const size_t smem = (size_t)(plan.warps + 2) * k * sizeof(int);
   KM_CUDA(allow_smem(sort_place_kernel, smem));
   sort_place_kernel<<<plan.blocks, kSortThreads, smem, stream>>>(ids, stride, n, entries, k, align, plan, part, offsets, counts, slot,
-                                                                 source, (long long)capacity);
+                                                                 source, (int)capacity);
   KM_CUDA(cudaGetLastError());
   return KM_OK;
 }
