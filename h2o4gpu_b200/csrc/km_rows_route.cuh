@@ -588,40 +588,55 @@ route_tile_kernel(const T* s, long long rs, long long cs, int rows, int k, int n
 // ---- the gradient ----------------------------------------------------------------------------------------------------------------------
 // Every score's own part first (zero over the taken alone), then the taken ones' over it.
 
+// An infinite score as the largest number of its sign; NaN stays.
+__device__ __forceinline__ float route_finite(float s) {
+  return s > 3.402823466e38f ? 3.402823466e38f : s < -3.402823466e38f ? -3.402823466e38f : s;
+}
+
 // One warp per row, 16-byte pieces.
-template <typename T, bool ALIGNED>
+template <typename T, bool ALIGNED, bool OVER_ALL>
 __global__ void __launch_bounds__(kRouteWarps * 32)
-route_grad_warp_kernel(const float* dweights, const T* s, long long rs, Span<T> in, int rows, int k, int n, float scale, bool over_all,
+route_grad_warp_kernel(const float* dweights, const T* s, long long rs, Span<T> in, int rows, int k, int n, float scale,
                        const int* ids, const float* weights, const float* best, const float* total, T* ds, long long drs) {
   constexpr int V = Piece<T>::V, H = V / 2;
   const int lane = threadIdx.x & 31, t = blockIdx.x * kRouteWarps + threadIdx.x / 32;
   if (t >= rows) return;
   int id = -1;
-  float w = 0.f, g = 0.f;
+  float w = 0.f, g = 0.f, b = 0.f, sum = 0.f;
   if (lane < n) {
     id = ids[(long long)t * n + lane];
     w = weights[(long long)t * n + lane];
     g = dweights[(long long)t * n + lane];
   }
+  if (OVER_ALL) {
+    b = best[t];
+    sum = total[t];
+  }
   const bool taken = id >= 0 && id < k;
-  const float c = warp_sum_f(taken ? w * g : 0.f);
+  const float c = warp_sum_f(taken ? w * g : 0.f), f = OVER_ALL && sum > 0.f ? -scale * c / sum : 0.f;
+  const bool huge = fabsf(b) == 3.402823466e38f;      // perhaps an infinite score, which counts as this
+  const T* sr = s + (long long)t * rs;
   T* dr = ds + (long long)t * drs;
-  const T* sr = over_all ? s + (long long)t * rs : nullptr;
-  const float sign = scale > 0.f ? 1.f : -1.f, a = fabsf(scale);
-  const float sum = over_all ? total[t] : 0.f, q0 = over_all ? sign * best[t] : 0.f, f = sum > 0.f ? -scale * c / sum : 0.f;
   const int pieces = ((k + V - 1) / V + 31) / 32 * 32;
+#pragma unroll 2
   for (int i = lane; i < pieces; i += 32) {
     Piece<T> p;
-    p.q = make_uint4(0u, 0u, 0u, 0u);
-    if (over_all) {
+    if (OVER_ALL) {
       p = load_piece<T, ALIGNED>(sr, i, k, in);
       float2 o[H];
+      unpack(p, o);
+      if (huge)
+#pragma unroll
+        for (int e = 0; e < H; ++e) o[e] = make_float2(route_finite(o[e].x), route_finite(o[e].y));
+      // |scale| (q - q_best) = scale (s - best); NaN and what cannot be taken give 0
 #pragma unroll
       for (int e = 0; e < H; ++e) {
-        const float qx = route_value(p.e[2 * e], sign), qy = route_value(p.e[2 * e + 1], sign);
-        o[e] = make_float2(qx > -INFINITY ? f * expf(a * (qx - q0)) : 0.f, qy > -INFINITY ? f * expf(a * (qy - q0)) : 0.f);
+        const float2 x = mul2(both(scale), add2(o[e], both(-b)));
+        o[e] = mul2(both(f), make_float2(expf(fmaxf(x.x, -INFINITY)), expf(fmaxf(x.y, -INFINITY))));
       }
       p = pack<T>(o);
+    } else {
+      p.q = make_uint4(0u, 0u, 0u, 0u);
     }
     store_piece<T, ALIGNED>(dr, i, k, p);
   }
@@ -755,10 +770,11 @@ int route_grad_launch(const float* dweights, const T* s, long long rs, long long
                       int sms, cudaStream_t stream) {
   if (dcs == 1 && (!over_all || cs == 1)) {
     const bool al = rows_aligned(ds, drs, rows, k, sizeof(T)) && (!over_all || rows_aligned(s, rs, rows, k, sizeof(T)));
-    const auto fn = al ? route_grad_warp_kernel<T, true> : route_grad_warp_kernel<T, false>;
+    const auto fn = over_all ? (al ? route_grad_warp_kernel<T, true, true> : route_grad_warp_kernel<T, false, true>)
+                             : (al ? route_grad_warp_kernel<T, true, false> : route_grad_warp_kernel<T, false, false>);
     fn<<<(rows + kRouteWarps - 1) / kRouteWarps, kRouteWarps * 32, 0, stream>>>(
-        dweights, s, rs, over_all ? span_of<T>(s, rs, rows, k) : Span<T>{nullptr, nullptr}, rows, k, n, scale, over_all, ids, weights,
-        best, total, ds, drs);
+        dweights, s, rs, over_all ? span_of<T>(s, rs, rows, k) : Span<T>{nullptr, nullptr}, rows, k, n, scale, ids, weights, best,
+        total, ds, drs);
     KM_CUDA(cudaGetLastError());
     return KM_OK;
   }

@@ -127,11 +127,13 @@ template <typename T>
 __device__ __forceinline__ Piece<T> load_window(const T* from, const Span<T>& in) {
   constexpr int V = Piece<T>::V;
   Piece<T> p;
-  const unsigned int off = (unsigned int)(reinterpret_cast<uintptr_t>(from) & 15);
-  const T* word = from - off / sizeof(T);
-  if (word >= in.lo && word + (off ? 2 * V : V) <= in.hi) {
-    const uint4 a = *reinterpret_cast<const uint4*>(word);
-    p.q = off ? shift_words(a, *reinterpret_cast<const uint4*>(word + V), off) : a;
+  const uintptr_t at = reinterpret_cast<uintptr_t>(from);
+  const unsigned int off = (unsigned int)(at & 15);
+  const uint4* word = reinterpret_cast<const uint4*>(at - off);
+  // (without an offset the second word is the first again)
+  const uint4* next = reinterpret_cast<const uint4*>((at + 15) & ~(uintptr_t)15);
+  if (reinterpret_cast<const T*>(word) >= in.lo && reinterpret_cast<const T*>(next + 1) <= in.hi) {
+    p.q = shift_words(*word, *next, off);
     return p;
   }
   p.q = make_uint4(0u, 0u, 0u, 0u);
