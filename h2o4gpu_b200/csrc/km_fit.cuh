@@ -665,6 +665,8 @@ int Engine<T>::nearest_shard(int local, int n, float scale, bool over_all, int* 
     KM_FAIL(KM_EINVAL, "kmeans_nearest_resident: bad argument");
   if (world_size != (int)shards.size()) KM_FAIL(KM_EINVAL, "kmeans_nearest_resident: handles of one process");
   if (!have_centroids) KM_FAIL(KM_ESTATE, "no centroids set");
+  // what it refuses of the arguments, before any distance
+  KM_TRY(kmeans_route(KM_DTYPE_F32, nullptr, 1, 1, 0, k, n, scale, over_all, nullptr, nullptr, nullptr, nullptr, nullptr));
   Shard<T>& s = shards[local];
   KM_TRY(distance_blocks(local, [&](size_t r, size_t nr, T* buf, size_t batch) -> int {
     return kmeans_route(KM_DTYPE_F32, buf, 1, (long long)batch, nr, k, n, scale, over_all, ids + r * n, weights + r * n, best + r,

@@ -230,7 +230,7 @@ route_lane_kernel(const T* s, long long rs, long long cs, int rows, int k, int n
   }
   const float q0 = first > -INFINITY ? first : 0.f;
   if (over_all) {
-    const float a2 = a * kLog2E;
+    const float a2 = fminf(a * kLog2E, 3.402823466e38f);
     walk([&](T r, int) { sum += exp2_fast(a2 * (route_value(r, sign) - q0)); }, [] {});
     if (split > 1) {
       __syncthreads();
@@ -329,7 +329,7 @@ route_warp_kernel(const T* s, long long rs, long long cs, Span<T> in, int rows, 
   }
   float sum = 0.f;
   if (over_all) {
-    const float2 a2 = both(a * kLog2E), off = both(-q0);
+    const float2 a2 = both(fminf(a * kLog2E, 3.402823466e38f)), off = both(-q0);
     float2 s2 = both(0.f);
     if (q0 < 3.402823466e38f) {
       walk([&](const float2 (&q)[V / 2], int) {
@@ -533,7 +533,7 @@ route_tile_kernel(const T* s, long long rs, long long cs, int rows, int k, int n
     end = list;
   };
   const float q0 = first > -INFINITY ? first : 0.f;
-  const float2 a2 = both(a * kLog2E), off = both(-q0);
+  const float2 a2 = both(fminf(a * kLog2E, 3.402823466e38f)), off = both(-q0);
   float2 s2 = both(0.f);
   for (int g = g0; g < g1; ++g) {
     float2 q[G / 2];

@@ -31,7 +31,7 @@ int layer_norm(int dtype, const void* x, long long xs, size_t rows, size_t cols,
                int param_dtype, double eps, void* y, long long ys, float* mean, float* rstd, cudaStream_t stream) {
   const int size = elem_size(dtype);
   if (!size) KM_FAIL(KM_EINVAL, "kmeans_layer_norm: rows are float32, float16 or bfloat16");
-  if (!(eps >= 0.0) || std::isinf(eps)) KM_FAIL(KM_EINVAL, "kmeans_layer_norm: eps must be finite and not negative");
+  if (!(eps >= 0.0) || !std::isfinite((float)eps)) KM_FAIL(KM_EINVAL, "kmeans_layer_norm: eps must be finite and not negative");
   KM_TRY(check_params("kmeans_layer_norm", dtype, cols, weight, bias, &param_dtype));
   if (rows == 0) return KM_OK;
   if (rows > kMaxRows || !block_ok(x, xs, rows, cols, size, false) || !block_ok(y, ys, rows, cols, size, true) ||

@@ -300,7 +300,8 @@ int kmeans_synth_f64(int gpu_id, double* dX, size_t rows, size_t cols, size_t ro
  * outputs and a workspace of its own.  Rows are float32, float16 or bfloat16 (KM_DTYPE_F32 / _F16 / _BF16), the
  * elements of a row side by side, rows `stride` elements apart (inputs may repeat a row with stride 0; outputs
  * may not overlap each other or an input, except where it says so).  Sums and statistics are float32; a value is rounded once,
- * when it is stored.  Results do not depend on the schedule: the same call gives the same bits.
+ * when it is stored.  Results do not depend on the schedule: the same call gives the same bits (of route's weights and
+ * total, and of dweights, on memory of the same strides and alignment).
  * Arguments are checked before anything is enqueued (KM_EINVAL); rows == 0 is valid and writes what has no rows.
  * Where `rows * n` entries or their places are counted, they are at most 0x7fff0000. */
 

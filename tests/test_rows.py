@@ -660,6 +660,99 @@ def test_layer_captured_in_two_graphs(built_lib):
 
 
 @gpu
+def test_captured_without_a_call_before(built_lib):
+    """A process whose first calls of the operators are captured ones."""
+    import subprocess
+    import sys
+    code = """
+import sys
+sys.path[:0] = [%r, %r]
+import torch
+from h2o4gpu_b200 import rows as R
+from test_rows import a_layer, layer_inputs
+v = layer_inputs(60)
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    out = a_layer(R, *v)
+g.replay()
+torch.cuda.synchronize()
+assert all(torch.equal(a, b) for a, b in zip(out, a_layer(R, *v)))
+print("as captured")
+"""
+    import os
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", code % (root, os.path.join(root, "tests"))], capture_output=True, text=True, timeout=300,
+                       cwd=root)
+    assert r.returncode == 0 and "as captured" in r.stdout, r.stderr[-2000:]
+
+
+@gpu
+def test_more_than_32_bits_of_elements(built_lib):
+    """Rows behind the 2^31st and 2^32nd byte and element come out as they do by themselves."""
+    R = rows_module(built_lib)
+    rows, d = 270_001, 8192                                   # 2.2e9 elements, 4.4 GB
+    if torch.cuda.mem_get_info()[0] < 16 << 30:
+        pytest.skip("needs 16 GB of free memory")
+    x = torch.empty((rows, d), dtype=torch.bfloat16, device="cuda")
+    x[:] = randn((1, d), 160, torch.bfloat16)
+    pick = torch.tensor([0, 131_071, 131_072, 262_143, 262_144, 262_145, 270_000], device="cuda")
+    x[pick] = randn((7, d), 161, torch.bfloat16)
+    small = x[pick]
+    y = R.layer_norm(x)
+    want = R.layer_norm(small)
+    assert torch.equal(y.y[pick], want.y) and torch.equal(y.mean[pick], want.mean)
+    g = R.layer_norm_grad(x, x, y.mean, y.rstd, params=False).dx[pick]
+    assert torch.equal(g, R.layer_norm_grad(small, small, want.mean, want.rstd, params=False).dx)
+    del y, g
+    ids = (torch.arange(rows, device="cuda", dtype=torch.int32) % 3).unsqueeze(1)
+    plan = R.sort_rows(ids, 3)
+    xs = R.dispatch(x, plan)
+    assert torch.equal(xs[plan.slot[pick, 0].long()], small)
+    assert torch.equal(R.dispatch_grad(xs, plan)[pick], small)
+    w = torch.ones((rows, 1), device="cuda")
+    dx, dw = R.combine_grad(x, xs, plan, w)
+    assert torch.equal(dx[plan.slot[pick, 0].long()], small)
+    square = (small.double() ** 2).sum(1)
+    within(dw[pick, 0], square, (d / 32 + 12) * U * square)
+    del xs, dx, x
+    torch.cuda.empty_cache()
+    k = 9000
+    s = torch.full((250_000, k), -5.0, dtype=torch.float16, device="cuda")        # 2.25e9 scores
+    best = torch.tensor([0, 119_304, 238_609, 249_999], device="cuda")
+    s[best, torch.tensor([5, 8999, 0, 77], device="cuda")] = 3.0
+    for v in (s, s.view(k, 250_000).t()):
+        if v is not s:
+            s.fill_(-5.0)
+            v[best, torch.tensor([5, 8999, 0, 77], device="cuda")] = 3.0
+        r = R.route(v, 1, 1.0)
+        assert r.ids[best, 0].tolist() == [5, 8999, 0, 77] and int((r.ids != 0).sum()) == 3
+        ds = R.route_grad(torch.ones_like(r.weights), v, r, 1.0)
+        assert ds.stride() == v.stride() and not bool(ds[best].any())            # one chosen: its weight is one whatever the score
+        del ds, r
+        r2 = R.route(v, 2, 1.0, "all")
+        assert r2.ids[best, 0].tolist() == [5, 8999, 0, 77]
+        ds = R.route_grad(torch.ones_like(r2.weights), v, r2, 1.0, "all")
+        few = R.route_grad(torch.ones((4, 2), device="cuda"), v[best].contiguous(),
+                           R.Routes(*[t[best].contiguous() for t in r2]), 1.0, "all")
+        # the same float32 value, but for a few roundings, rounded once on either side
+        assert bool(((ds[best] - few).float().abs() <= 4 * half(torch.float16) * few.float().abs() + 2 * tiny(torch.float16)).all())
+        del ds, r2
+
+
+@gpu
+def test_route_with_the_largest_scales(built_lib):
+    R = rows_module(built_lib)
+    s = make_scores(40, 200, torch.float32, 170, masked=False)
+    s[:, 7] = s[:, 3]
+    for scale in (HUGE, -HUGE, 2.0 ** -126):
+        for n in (1, 4, 12):
+            for over in ("chosen", "all"):
+                for v in (s, s.t().contiguous().t()):
+                    check_route(R, v, n, scale, over)
+
+
+@gpu
 def test_layer_on_another_device_than_the_current_one(built_lib):
     if torch.cuda.device_count() < 2:
         pytest.skip("needs two devices")
@@ -812,7 +905,7 @@ def test_c_refuses_bad_arguments_before_any_device_call(built_lib):
 
     big = 1 << 40
     bad = [norm(dtype=1), norm(dtype=3), norm(dtype=99), norm(x=None), norm(x=odd), norm(xs=-1), norm(cols=0), norm(ys=7), norm(y=None),
-           norm(w=p, pd=2), norm(w=odd), norm(eps=-1.0), norm(eps=nan), norm(eps=float("inf")), norm(rows=big), norm(cols=big),
+           norm(w=p, pd=2), norm(w=odd), norm(eps=-1.0), norm(eps=nan), norm(eps=float("inf")), norm(eps=1e300), norm(rows=big), norm(cols=big),
            norm(mean=odd), norm(xs=big),
            norm_grad(dtype=1), norm_grad(dy=None), norm_grad(dw=None), norm_grad(dx=odd), norm_grad(dxs=4), norm_grad(mean=None),
            norm_grad(rows=big), norm_grad(w=p, pd=11),
