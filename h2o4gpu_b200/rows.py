@@ -23,6 +23,7 @@ from .libs import lib_kmeans as _lk
 
 _CODES = {torch.float32: 0, torch.float16: 2, torch.bfloat16: 11}
 _OVER = {"chosen": 0, "all": 1}
+_SORT_ONE_CTA = 2048      # entries below which kmeans_sort_rows needs no workspace
 
 
 class LayerNorm(NamedTuple):
@@ -100,57 +101,64 @@ def _sizes(fn, index, *args):
         _lk.check(rc)
 
 
-def _refuse(name, t, device=None, dtype=None, shape=None):
-    """Raises what is wrong with a tensor that should be on `device`, of `dtype` and `shape` (where they are given)."""
+def _refuse(name, t, index=None, dtype=None, shape=None):
+    """Raises what is wrong with a tensor that should be on device `index`, of `dtype` and `shape` (where they are given)."""
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
         raise ValueError("%s must be a CUDA tensor" % name)
-    if device is not None and t.device != device:
-        raise ValueError("%s is on %s, not on %s" % (name, t.device, device))
+    if index is not None and t.get_device() != index:
+        raise ValueError("%s is on %s, not on cuda:%d" % (name, t.device, index))
     if dtype is not None and t.dtype != dtype:
         raise ValueError("%s must be %s, not %s" % (name, dtype, t.dtype))
     if dtype is None and t.dtype not in _CODES:
         raise ValueError("%s must be float32, float16 or bfloat16, not %s" % (name, t.dtype))
     if shape is not None and t.shape != shape:
         raise ValueError("%s has shape %s, not %s" % (name, tuple(t.shape), tuple(shape)))
+    if shape is None and t.dim() != 2:
+        raise ValueError("%s must be two-dimensional" % name)
     raise ValueError("%s: the elements must lie side by side" % name)
 
 
+# The checks below ask a tensor for as little as they can: they are a good part of a small call's time.
+
 def _rows(name, t):
-    """(rows, cols, row stride, type code) of a two-dimensional tensor whose rows have their elements side by side."""
-    if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dtype not in _CODES:
+    """(rows, cols, row stride, type code, device) of a two-dimensional tensor whose rows have their elements side by side."""
+    try:
+        code, index = _CODES[t.dtype], t.get_device()
+        rows, cols = t.shape
+        stride, inner = t.stride()
+    except (AttributeError, KeyError, ValueError):
         _refuse(name, t)
-    if t.dim() != 2:
-        raise ValueError("%s must be two-dimensional" % name)
-    rows, cols = t.shape
-    stride, inner = t.stride()
-    if inner != 1 and cols > 1:
-        raise ValueError("%s: the elements of a row must lie side by side" % name)
-    return rows, cols, stride if rows > 1 else cols, _CODES[t.dtype]
+    if index < 0 or (inner != 1 and cols > 1):
+        _refuse(name, t)
+    return rows, cols, stride if rows > 1 else cols, code, index
 
 
-def _same_rows(name, t, like, shape):
-    """Row stride of such a tensor that has `shape` and is `like` another in type and device."""
-    if not isinstance(t, torch.Tensor) or t.dtype != like.dtype or t.device != like.device or t.shape != shape:
-        _refuse(name, t, like.device, like.dtype, shape)
+def _same_rows(name, t, like, index, shape):
+    """Row stride of such a tensor that has `shape`, `like`'s type and its device."""
+    if not isinstance(t, torch.Tensor) or t.dtype is not like.dtype or t.get_device() != index or t.shape != shape:
+        _refuse(name, t, index, like.dtype, shape)
     stride, inner = t.stride()
     if inner != 1 and shape[1] > 1:
-        raise ValueError("%s: the elements of a row must lie side by side" % name)
+        _refuse(name, t, index, like.dtype, shape)
     return stride if shape[0] > 1 else shape[1]
 
 
-def _flat(name, t, device, dtype, shape):
-    """Address of a contiguous tensor of this type and shape."""
-    if not isinstance(t, torch.Tensor) or t.dtype != dtype or t.device != device or t.shape != shape or not t.is_contiguous():
-        _refuse(name, t, device, dtype, shape)
-    return t.data_ptr()
+def _flat(name, t, index, dtype, shape):
+    """Address of a contiguous tensor of this type and shape on this device."""
+    try:
+        if t.dtype is dtype and t.get_device() == index and t.shape == shape and t.is_contiguous():
+            return t.data_ptr()
+    except AttributeError:
+        pass
+    _refuse(name, t, index, dtype, shape)
 
 
-def _out(out, like, rows, cols, exact=True):
+def _out(out, like, index, rows, cols, exact=True):
     """The caller's output, or a new one of `like`'s type and device; and its row stride."""
     if out is None:
         return like.new_empty((rows, cols)), cols
     have = out.shape[0] if isinstance(out, torch.Tensor) and out.dim() == 2 else rows
-    return out, _same_rows("out", out, like, (rows if exact or have < rows else have, cols))
+    return out, _same_rows("out", out, like, index, (rows if exact or have < rows else have, cols))
 
 
 def _over(over):
@@ -161,65 +169,73 @@ def _over(over):
 
 # ---- layer norm ------------------------------------------------------------------------------------------------------
 
-def _param(name, t, x, cols):
+def _param(name, t, x, index, cols):
     """Address and type code of a weight or bias."""
-    if not isinstance(t, torch.Tensor) or t.dtype not in (torch.float32, x.dtype):
+    dtype = getattr(t, "dtype", None)
+    if dtype is not x.dtype and dtype is not torch.float32:
         raise ValueError("%s must be float32 or of the rows' type" % name)
-    return _flat(name, t, x.device, t.dtype, (cols,)), _CODES[t.dtype]
+    return _flat(name, t, index, dtype, (cols,)), _CODES[dtype]
 
 
 def layer_norm(x, weight=None, bias=None, eps=1e-5, out=None):
     """(x - mean) / sqrt(variance + eps) * weight + bias of each row of x (rows, cols); weight and bias (cols, float32
     or x's type, both the same) may be left out.  `out` may be x."""
-    rows, cols, stride, code = _rows("x", x)
+    rows, cols, stride, code, index = _rows("x", x)
     w = b = None
     pcode = 0
     if weight is not None:
-        w, pcode = _param("weight", weight, x, cols)
+        w, pcode = _param("weight", weight, x, index, cols)
     if bias is not None:
-        b, bcode = _param("bias", bias, x, cols)
+        b, bcode = _param("bias", bias, x, index, cols)
         if weight is not None and bcode != pcode:
             raise ValueError("weight and bias must be of one type")
         pcode = bcode
-    y, ystride = _out(out, x, rows, cols)
+    if out is None and stride == cols:
+        y, ystride = torch.empty_like(x), cols
+    else:
+        y, ystride = _out(out, x, index, rows, cols)
     mean = x.new_empty(rows, dtype=torch.float32)
     rstd = torch.empty_like(mean)
-    _call(_lib.kmeans_layer_norm, x.get_device(), code, x.data_ptr(), stride, rows, cols, w, b, pcode, eps, y.data_ptr(), ystride,
+    _call(_lib.kmeans_layer_norm, index, code, x.data_ptr(), stride, rows, cols, w, b, pcode, eps, y.data_ptr(), ystride,
           mean.data_ptr(), rstd.data_ptr())
     return LayerNorm(y, mean, rstd)
 
 
 def layer_norm_grad(dy, x, mean, rstd, weight=None, params=True):
     """Gradient of :func:`layer_norm`: dx, and with `params` the float32 gradients of weight and bias."""
-    rows, cols, stride, code = _rows("x", x)
-    dev, index = x.device, x.get_device()
-    dstride = _same_rows("dy", dy, x, x.shape)
-    m = _flat("mean", mean, dev, torch.float32, (rows,))
-    r = _flat("rstd", rstd, dev, torch.float32, (rows,))
-    w, pcode = (None, 0) if weight is None else _param("weight", weight, x, cols)
-    dx = x.new_empty((rows, cols))
-    dweight = dbias = ws = None
+    rows, cols, stride, code, index = _rows("x", x)
+    dstride = _same_rows("dy", dy, x, index, x.shape)
+    m = _flat("mean", mean, index, torch.float32, (rows,))
+    r = _flat("rstd", rstd, index, torch.float32, (rows,))
+    w, pcode = (None, 0) if weight is None else _param("weight", weight, x, index, cols)
+    dx = torch.empty_like(x) if stride == cols else x.new_empty((rows, cols))
+    if not params:
+        _call(_lib.kmeans_layer_norm_grad, index, code, dy.data_ptr(), dstride, x.data_ptr(), stride, m, r, rows, cols, w, pcode,
+              dx.data_ptr(), cols, None, None, None, 0)
+        return LayerNormGrad(dx, None, None)
+    dweight = x.new_empty(cols, dtype=torch.float32)
+    dbias = torch.empty_like(dweight)
     size = ctypes.c_size_t(0)
-    if params:
-        dweight = x.new_empty(cols, dtype=torch.float32)
-        dbias = torch.empty_like(dweight)
-        _sizes(_lib.kmeans_layer_norm_grad_workspace, index, rows, cols, ctypes.byref(size))
-        ws = x.new_empty(size.value, dtype=torch.uint8)
+    _sizes(_lib.kmeans_layer_norm_grad_workspace, index, rows, cols, ctypes.byref(size))
+    ws = x.new_empty(size.value, dtype=torch.uint8)
     _call(_lib.kmeans_layer_norm_grad, index, code, dy.data_ptr(), dstride, x.data_ptr(), stride, m, r, rows, cols, w, pcode,
-          dx.data_ptr(), cols, dweight.data_ptr() if params else None, dbias.data_ptr() if params else None,
-          ws.data_ptr() if params else None, size.value)
+          dx.data_ptr(), cols, dweight.data_ptr(), dbias.data_ptr(), ws.data_ptr(), size.value)
     return LayerNormGrad(dx, dweight, dbias)
 
 
 # ---- routing ---------------------------------------------------------------------------------------------------------
 
 def _scores(scores):
-    """(rows, clusters, their strides, type code) of two-dimensional scores in any strides."""
-    if not isinstance(scores, torch.Tensor) or not scores.is_cuda or scores.dtype not in _CODES:
+    """(rows, clusters, their strides, type code, device) of two-dimensional scores in any strides."""
+    try:
+        code, index = _CODES[scores.dtype], scores.get_device()
+        rows, k = scores.shape
+        rs, cs = scores.stride()
+    except (AttributeError, KeyError, ValueError):
         _refuse("scores", scores)
-    if scores.dim() != 2:
-        raise ValueError("scores must be two-dimensional")
-    return (*scores.shape, *scores.stride(), _CODES[scores.dtype])
+    if index < 0:
+        _refuse("scores", scores)
+    return rows, k, rs, cs, code, index
 
 
 def _routes(rows, n, like):
@@ -236,11 +252,11 @@ def route(scores, n, scale=-1.0, over="chosen"):
     scale > 0: larger scores are better, scale < 0: smaller ones (distances; -1 / temperature).  The weights are a softmax
     of scale * score over the chosen clusters, or over all of them (`over`).  Ties go to the lowest cluster; NaN and infinitely
     bad scores are never chosen."""
-    rows, k, rs, cs, code = _scores(scores)
+    rows, k, rs, cs, code, index = _scores(scores)
     flag = _over(over)
     out = _routes(rows, n, scores)
     ids, weights, best, total = out
-    _call(_lib.kmeans_route, scores.get_device(), code, scores.data_ptr(), rs, cs, rows, k, n, scale, flag, ids.data_ptr(),
+    _call(_lib.kmeans_route, index, code, scores.data_ptr(), rs, cs, rows, k, n, scale, flag, ids.data_ptr(),
           weights.data_ptr(), best.data_ptr(), total.data_ptr())
     return out
 
@@ -248,22 +264,22 @@ def route(scores, n, scale=-1.0, over="chosen"):
 def route_grad(dweights, scores, routes, scale=-1.0, over="chosen"):
     """Gradient of the scores, of their type and in their order of dimensions, from that of the weights; `routes`, `scale`
     and `over` as :func:`route` returned and took them."""
-    rows, k, rs, cs, code = _scores(scores)
+    rows, k, rs, cs, code, index = _scores(scores)
     flag = _over(over)
     ids, weights, best, total = routes
     if ids.dim() != 2:
         raise ValueError("routes.ids must be two-dimensional")
-    dev, n = scores.device, ids.shape[1]
-    f32, shape = torch.float32, (rows, n)
-    args = (_flat("routes.ids", ids, dev, torch.int32, shape), _flat("routes.weights", weights, dev, f32, shape),
-            _flat("routes.best", best, dev, f32, (rows,)), _flat("routes.total", total, dev, f32, (rows,)))
+    n, f32 = ids.shape[1], torch.float32
+    shape = (rows, n)
+    args = (_flat("routes.ids", ids, index, torch.int32, shape), _flat("routes.weights", weights, index, f32, shape),
+            _flat("routes.best", best, index, f32, (rows,)), _flat("routes.total", total, index, f32, (rows,)))
     if rs < cs:
         out = scores.new_empty((k, rows)).t()
         drs, dcs = 1, rows
     else:
         out = scores.new_empty((rows, k))
         drs, dcs = k, 1
-    _call(_lib.kmeans_route_grad, scores.get_device(), code, _flat("dweights", dweights, dev, f32, shape), scores.data_ptr(), rs, cs,
+    _call(_lib.kmeans_route_grad, index, code, _flat("dweights", dweights, index, f32, shape), scores.data_ptr(), rs, cs,
           rows, k, n, scale, flag, *args, out.data_ptr(), drs, dcs)
     return out
 
@@ -283,7 +299,7 @@ def nearest(handle, n, scale=-1.0, over="chosen", local=0):
 def sort_rows(ids, k, align=1):
     """Places of rows sorted by cluster: ids (rows,) or (rows, n) int32, outside [0, k) for entries that go nowhere.  Groups
     start on multiples of `align`; entries of a group keep their order."""
-    if not isinstance(ids, torch.Tensor) or not ids.is_cuda or ids.dtype != torch.int32:
+    if not isinstance(ids, torch.Tensor) or not ids.is_cuda or ids.dtype is not torch.int32:
         _refuse("ids", ids, None, torch.int32)
     if ids.dim() == 1:
         ids = ids.unsqueeze(1)
@@ -293,39 +309,43 @@ def sort_rows(ids, k, align=1):
     stride, inner = ids.stride()
     if inner != 1 and n > 1:
         raise ValueError("ids: the elements of a row must lie side by side")
-    index = ids.get_device()
-    capacity, size = ctypes.c_size_t(0), ctypes.c_size_t(0)
-    _sizes(_lib.kmeans_sort_rows_sizes, index, rows, n, k, align, ctypes.byref(capacity), ctypes.byref(size))
+    index, entries = ids.get_device(), rows * n
+    places, work = entries + min(k, entries) * (align - 1), 0
+    if entries >= _SORT_ONE_CTA:
+        capacity, size = ctypes.c_size_t(0), ctypes.c_size_t(0)
+        _sizes(_lib.kmeans_sort_rows_sizes, index, rows, n, k, align, ctypes.byref(capacity), ctypes.byref(size))
+        places, work = capacity.value, size.value
     offsets = ids.new_empty(k + 1)
     counts = ids.new_empty(k)
     slot = ids.new_empty((rows, n))
-    source = ids.new_empty(capacity.value)
-    ws = ids.new_empty(size.value, dtype=torch.uint8) if size.value else None
+    source = ids.new_empty(places)
+    ws = ids.new_empty(work, dtype=torch.uint8) if work else None
     _call(_lib.kmeans_sort_rows, index, ids.data_ptr(), stride if rows > 1 else n, rows, n, k, align, offsets.data_ptr(),
-          counts.data_ptr(), slot.data_ptr(), source.data_ptr(), None if ws is None else ws.data_ptr(), size.value)
+          counts.data_ptr(), slot.data_ptr(), source.data_ptr(), ws.data_ptr() if work else None, work)
     return SortedRows(offsets, counts, slot, source)
 
 
-def _plan(plan, dev):
+def _plan(plan, index):
     """(address of slot, address of source, rows, entries a row, places)"""
     slot, source = plan.slot, plan.source
-    if slot.dim() != 2 or source.dim() != 1:
-        raise ValueError("plan.slot must be two-dimensional and plan.source one-dimensional")
-    rows, n = slot.shape
-    return (_flat("plan.slot", slot, dev, torch.int32, slot.shape), _flat("plan.source", source, dev, torch.int32, source.shape),
-            rows, n, source.shape[0])
+    try:
+        rows, n = slot.shape
+        places, = source.shape
+    except ValueError:
+        raise ValueError("plan.slot must be two-dimensional and plan.source one-dimensional") from None
+    return (_flat("plan.slot", slot, index, torch.int32, slot.shape), _flat("plan.source", source, index, torch.int32, source.shape),
+            rows, n, places)
 
 
 def dispatch(x, plan, out=None):
     """Rows of x (rows, cols) at the places of `plan` (places, cols); padding becomes zero rows.  `out` may have more
     rows than the plan has places: those behind stay as they are."""
-    have, cols, stride, code = _rows("x", x)
-    slot, source, rows, n, capacity = _plan(plan, x.device)
+    have, cols, stride, code, index = _rows("x", x)
+    slot, source, rows, n, places = _plan(plan, index)
     if have != rows:
         raise ValueError("x has %d rows, the plan %d" % (have, rows))
-    y, ystride = _out(out, x, capacity, cols, exact=False)
-    _call(_lib.kmeans_dispatch, x.get_device(), code, x.data_ptr(), stride, rows, cols, n, slot, source, capacity, y.data_ptr(),
-          ystride)
+    y, ystride = _out(out, x, index, places, cols, exact=False)
+    _call(_lib.kmeans_dispatch, index, code, x.data_ptr(), stride, rows, cols, n, slot, source, places, y.data_ptr(), ystride)
     return y
 
 
@@ -337,26 +357,26 @@ def dispatch_grad(drows, plan, out=None):
 def combine(rows, plan, weights=None, out=None):
     """Sum of each row's entries of the sorted `rows` (places, cols), with weights (rows, n) float32 or without; entries
     that went nowhere add nothing."""
-    have, cols, stride, code = _rows("rows", rows)
-    slot, _, t, n, capacity = _plan(plan, rows.device)
-    if have < capacity:
-        raise ValueError("rows has %d rows, the plan %d places" % (have, capacity))
-    w = None if weights is None else _flat("weights", weights, rows.device, torch.float32, (t, n))
-    y, ystride = _out(out, rows, t, cols)
-    _call(_lib.kmeans_combine, rows.get_device(), code, rows.data_ptr(), stride, capacity, cols, slot, w, t, n, y.data_ptr(), ystride)
+    have, cols, stride, code, index = _rows("rows", rows)
+    slot, _, t, n, places = _plan(plan, index)
+    if have < places:
+        raise ValueError("rows has %d rows, the plan %d places" % (have, places))
+    w = None if weights is None else _flat("weights", weights, index, torch.float32, (t, n))
+    y, ystride = _out(out, rows, index, t, cols)
+    _call(_lib.kmeans_combine, index, code, rows.data_ptr(), stride, places, cols, slot, w, t, n, y.data_ptr(), ystride)
     return y
 
 
 def combine_grad(dy, rows, plan, weights):
     """Gradients of :func:`combine` for the sorted rows (zero rows at padding) and the weights."""
-    have, cols, stride, code = _rows("rows", rows)
-    slot, source, t, n, capacity = _plan(plan, rows.device)
-    if have < capacity:
-        raise ValueError("rows has %d rows, the plan %d places" % (have, capacity))
-    dstride = _same_rows("dy", dy, rows, (t, cols))
-    w = _flat("weights", weights, rows.device, torch.float32, (t, n))
-    drows = rows.new_empty((capacity, cols))
+    have, cols, stride, code, index = _rows("rows", rows)
+    slot, source, t, n, places = _plan(plan, index)
+    if have < places:
+        raise ValueError("rows has %d rows, the plan %d places" % (have, places))
+    dstride = _same_rows("dy", dy, rows, index, (t, cols))
+    w = _flat("weights", weights, index, torch.float32, (t, n))
+    drows = rows.new_empty((places, cols))
     dweights = torch.empty_like(weights)
-    _call(_lib.kmeans_combine_grad, rows.get_device(), code, dy.data_ptr(), dstride, rows.data_ptr(), stride, capacity, cols, slot,
-          source, w, t, n, drows.data_ptr(), cols, dweights.data_ptr())
+    _call(_lib.kmeans_combine_grad, index, code, dy.data_ptr(), dstride, rows.data_ptr(), stride, places, cols, slot, source, w, t, n,
+          drows.data_ptr(), cols, dweights.data_ptr())
     return CombineGrad(drows, dweights)

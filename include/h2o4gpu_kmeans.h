@@ -354,7 +354,8 @@ int kmeans_nearest_resident(kmeans_handle_t h, int local, int n, float scale, in
  *   offsets[k + 1]  where each cluster's group starts; offsets[k] = places in use, padding included
  *   counts[k]       entries of each cluster
  *   slot[rows * n]  place of entry row * n + j, or -1
- *   source[capacity] entry at a place, or -1 for padding and unused places */
+ *   source[capacity] entry at a place, or -1 for padding and unused places
+ * Fewer than 2048 entries need no workspace. */
 int kmeans_sort_rows_sizes(size_t rows, int n, int k, int align, size_t* capacity, size_t* workspace_bytes);
 int kmeans_sort_rows(const int32_t* ids, long long ids_stride, size_t rows, int n, int k, int align,
                      int32_t* offsets, int32_t* counts, int32_t* slot, int32_t* source, void* workspace,
