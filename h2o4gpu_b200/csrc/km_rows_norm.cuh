@@ -11,15 +11,16 @@ namespace rows {
 
 constexpr int kNormThreads = 256;   // of the kernels for wide rows
 
-// Weights or biases of the columns of piece i (2 H of them), `none` behind the row's end.  They stay in L1 from row to row.
-template <typename P, int H, bool ALIGNED>
-__device__ __forceinline__ void load_params(const P* w, int i, int d, bool inside, float none, float2 (&f)[H]) {
+// Weights or biases of the columns of piece i (2 H of them), `none` behind the row's end.  They stay in L1 from row to row.  WHOLE: they
+// start on a 16-byte boundary and the row is whole pieces; else `words` says whether they start on one.
+template <typename P, int H, bool WHOLE>
+__device__ __forceinline__ void load_params(const P* w, int i, int d, bool inside, bool words, float none, float2 (&f)[H]) {
   constexpr int V = 2 * H;
   const int c = i * V;
 #pragma unroll
   for (int e = 0; e < H; ++e) f[e] = both(none);
   if (!inside) return;
-  if (ALIGNED) {      // of whole pieces
+  if (WHOLE || (words && c + V <= d)) {
     constexpr int PV = Piece<P>::V;
 #pragma unroll
     for (int h = 0; h < V / PV; ++h) {
@@ -87,6 +88,7 @@ norm_rows_kernel(const T* x, long long xs, Span<T> xin, int rows, int d, float i
   constexpr int V = Piece<T>::V, H = V / 2;
   __shared__ float2 red[2][16];      // used in turn: one half may still be read by slower warps
   const int in_group = threadIdx.x, lane = threadIdx.x & 31, warps = blockDim.x / 32;
+  const bool w_words = (reinterpret_cast<uintptr_t>(w) & 15) == 0, b_words = (reinterpret_cast<uintptr_t>(b) & 15) == 0;
   // warp i of the group has the 32 NV pieces from i * 32 NV on, each lane every 32nd of them
   const auto columns = [&](int i) { return (float)max(0, min(32 * NV * V, d - i * 32 * NV * V)); };
   const int first = in_group / 32 * (32 * NV) + lane;
@@ -146,8 +148,8 @@ norm_rows_kernel(const T* x, long long xs, Span<T> xin, int rows, int d, float i
       for (int p = 0; p < NV; ++p) {
         const int i = first + p * 32;
         float2 wf[H], bf[H];
-        if (with_w()) load_params<P, H, ALIGNED>(w, i, d, p < have, 1.f, wf);
-        if (with_b()) load_params<P, H, ALIGNED>(b, i, d, p < have, 0.f, bf);
+        if (with_w()) load_params<P, H, ALIGNED>(w, i, d, p < have, w_words, 1.f, wf);
+        if (with_b()) load_params<P, H, ALIGNED>(b, i, d, p < have, b_words, 0.f, bf);
 #pragma unroll
         for (int e = 0; e < H; ++e) {
           float2 o = mul2(add2(v[p][e], both(-mu)), both(r));
@@ -205,6 +207,7 @@ norm_grad_rows_kernel(const T* dy, long long dys, Span<T> gin, const T* x, long 
   extern __shared__ uint4 ring[];   // [warp][S][x, dy][NV][lane]; in the end the CTA's sums
   const int group = blockDim.x, per_cta = blockDim.y, which = threadIdx.y, in_group = threadIdx.x, lane = threadIdx.x & 31;
   const int warps = group / 32;
+  const bool w_words = (reinterpret_cast<uintptr_t>(w) & 15) == 0;
   const int first = in_group / 32 * (32 * NV) + lane;      // as in norm_rows_kernel
   const int have = min(NV, max(0, ((d + V - 1) / V - first + 31) / 32));
   float2 aw[NV][H], ab[NV][H];
@@ -252,7 +255,7 @@ norm_grad_rows_kernel(const T* dy, long long dys, Span<T> gin, const T* x, long 
 #pragma unroll
       for (int p = 0; p < NV; ++p) {
         float2 wf[H];
-        if (with_w()) load_params<P, H, ALIGNED>(w, first + p * 32, d, p < have, 1.f, wf);
+        if (with_w()) load_params<P, H, ALIGNED>(w, first + p * 32, d, p < have, w_words, 1.f, wf);
 #pragma unroll
         for (int e = 0; e < H; ++e) {
           xh[p][e] = fma2(xh[p][e], rr, off);     // behind the row's end g is zero

@@ -127,13 +127,15 @@ template <typename T>
 __device__ __forceinline__ Piece<T> load_window(const T* from, const Span<T>& in) {
   constexpr int V = Piece<T>::V;
   Piece<T> p;
-  const uintptr_t at = reinterpret_cast<uintptr_t>(from);
-  const unsigned int off = (unsigned int)(at & 15);
-  const uint4* word = reinterpret_cast<const uint4*>(at - off);
-  // (without an offset the second word is the first again)
-  const uint4* next = reinterpret_cast<const uint4*>((at + 15) & ~(uintptr_t)15);
-  if (reinterpret_cast<const T*>(word) >= in.lo && reinterpret_cast<const T*>(next + 1) <= in.hi) {
-    p.q = shift_words(*word, *next, off);
+  const unsigned int off = (unsigned int)(reinterpret_cast<uintptr_t>(from) & 15);
+  const T* word = from - off / sizeof(T);
+  if (off == 0) {      // (as a rule the same for a whole row)
+    if (from >= in.lo && from + V <= in.hi) {
+      p.q = *reinterpret_cast<const uint4*>(from);
+      return p;
+    }
+  } else if (word >= in.lo && word + 2 * V <= in.hi) {
+    p.q = shift_words(*reinterpret_cast<const uint4*>(word), *reinterpret_cast<const uint4*>(word + V), off);
     return p;
   }
   p.q = make_uint4(0u, 0u, 0u, 0u);
