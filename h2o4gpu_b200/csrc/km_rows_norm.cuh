@@ -43,13 +43,25 @@ __device__ __forceinline__ void load_params(const P* w, int i, int d, bool insid
 template <typename T, int NV, bool ALIGNED>
 __device__ __forceinline__ void load_pieces(const T* row, int first, int have, int d, const Span<T>& in, Piece<T> (&p)[NV]) {
   const uint4* q = reinterpret_cast<const uint4*>(row) + first;
+  if (ALIGNED) {
 #pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    if (ALIGNED) {
+    for (int i = 0; i < NV; ++i)
       if (i < have) p[i].q = q[i * 32];
-    } else {
-      p[i] = load_piece<T, false>(row, first + i * 32, d, in);
+  } else if (words_inside(row, d, in)) {      // all rows but a block's first and last
+    constexpr int V = Piece<T>::V;
+    const int m = before_row(row);
+    const uint4* word = reinterpret_cast<const uint4*>(row - m) + first;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = (first + i * 32) * V;
+      if (c >= d) continue;
+      const uint4 a = word[i * 32];
+      p[i].q = m && c + V - m < d ? shift_words(a, word[i * 32 + 1], m * (int)sizeof(T)) : shift_words(a, a, m * (int)sizeof(T));
+      clip_piece(p[i], c, d);
     }
+  } else {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) p[i] = load_piece<T, false>(row, first + i * 32, d, in);
   }
 }
 
@@ -144,6 +156,7 @@ norm_rows_kernel(const T* x, long long xs, Span<T> xin, int rows, int d, float i
     T* yr = y + (long long)t * ys;
     const auto finish = [&](auto with_w, auto with_b) {
       uint4* out = reinterpret_cast<uint4*>(yr) + first;
+      Piece<T> done[NV];
 #pragma unroll
       for (int p = 0; p < NV; ++p) {
         const int i = first + p * 32;
@@ -161,9 +174,10 @@ norm_rows_kernel(const T* x, long long xs, Span<T> xin, int rows, int d, float i
         if (ALIGNED) {
           if (p < have) out[p * 32] = pack<T>(v[p]).q;
         } else {
-          store_piece<T, false>(yr, i, d, pack<T>(v[p]));
+          done[p] = pack<T>(v[p]);
         }
       }
+      if (!ALIGNED) store_pieces(yr, first, d, done);
     };
     using std::integral_constant;
     if (w && b) finish(integral_constant<bool, true>(), integral_constant<bool, true>());
@@ -204,7 +218,8 @@ norm_grad_rows_kernel(const T* dy, long long dys, Span<T> gin, const T* x, long 
                       float inv_d, const P* w, T* dx, long long dxs, float* part) {
   constexpr int V = Piece<T>::V, H = V / 2, S = norm_grad_ahead<NV>();
   __shared__ float2 red[2][8];      // used in turn: one half may still be read by slower warps
-  extern __shared__ uint4 ring[];   // [warp][S][x, dy][NV][lane]; in the end the CTA's sums
+  constexpr int WORDS = NV * 32 + (ALIGNED ? 0 : 1);      // of a warp's share of a row; unaligned, its last piece ends one further
+  extern __shared__ uint4 ring[];   // [warp][S][x, dy][WORDS]; in the end the CTA's sums
   const int group = blockDim.x, per_cta = blockDim.y, which = threadIdx.y, in_group = threadIdx.x, lane = threadIdx.x & 31;
   const int warps = group / 32;
   const bool w_words = (reinterpret_cast<uintptr_t>(w) & 15) == 0;
@@ -221,25 +236,49 @@ norm_grad_rows_kernel(const T* dy, long long dys, Span<T> gin, const T* x, long 
     Piece<T> x[NV], g[NV];
     float mu, r;
   };
-  uint4* slots = ring + (which * warps + in_group / 32) * (S * 2 * NV * 32) + lane;
-  const auto copy = [&](int row, int slot) {      // ALIGNED: starts the copies of a row
-    if (row < rows) {
-      const uint4* xq = reinterpret_cast<const uint4*>(x + (long long)row * xs) + first;
-      const uint4* gq = reinterpret_cast<const uint4*>(dy + (long long)row * dys) + first;
-      uint4* to = slots + slot * (2 * NV * 32);
+  uint4* slots = ring + (which * warps + in_group / 32) * (S * 2 * WORDS);
+  // starts the copies of one of a row's two blocks; unaligned: of the words that its pieces lie across
+  const auto copy_block = [&](const T* from, uint4* to) {
+    if (ALIGNED) {
+      const uint4* q = reinterpret_cast<const uint4*>(from) + first;
 #pragma unroll
       for (int p = 0; p < NV; ++p)
-        if (p < have) {
-          copy_async(to + p * 32, xq + p * 32);
-          copy_async(to + (NV + p) * 32, gq + p * 32);
-        }
+        if (p < have) copy_async(to + p * 32 + lane, q + p * 32);
+    } else {
+      const int m = before_row(from), words = (m + d + V - 1) / V;
+      const uint4* q = reinterpret_cast<const uint4*>(from - m);
+#pragma unroll
+      for (int p = 0; p < NV; ++p)
+        if (first + p * 32 < words) copy_async(to + p * 32 + lane, q + first + p * 32);
+      if (lane == 0 && first + NV * 32 < words) copy_async(to + NV * 32, q + first + NV * 32);
+    }
+  };
+  const auto copy = [&](int row, int slot) {
+    if (row < rows) {
+      const T* xr = x + (long long)row * xs;
+      const T* gr = dy + (long long)row * dys;
+      uint4* to = slots + slot * (2 * WORDS);
+      if (ALIGNED || words_inside(xr, d, xin)) copy_block(xr, to);
+      if (ALIGNED || words_inside(gr, d, gin)) copy_block(gr, to + WORDS);
     }
     copies_commit();
   };
-  const auto load = [&](int row, Row& to) {       // not ALIGNED: the row itself
-    if (row >= rows) return;
-    load_pieces<T, NV, ALIGNED>(x + (long long)row * xs, first, have, d, xin, to.x);
-    load_pieces<T, NV, ALIGNED>(dy + (long long)row * dys, first, have, d, gin, to.g);
+  const auto take = [&](const T* from, const uint4* at, const Span<T>& in, Piece<T>(&p)[NV]) {
+    if (ALIGNED) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) p[i].q = at[i * 32 + lane];
+    } else if (words_inside(from, d, in)) {
+      const int off = before_row(from) * (int)sizeof(T);
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int c = (first + i * 32) * V;
+        p[i].q = c < d ? shift_words(at[i * 32 + lane], at[i * 32 + lane + 1], off) : make_uint4(0u, 0u, 0u, 0u);
+        if (c < d) clip_piece(p[i], c, d);
+      }
+    } else {      // a block's first or last row
+#pragma unroll
+      for (int i = 0; i < NV; ++i) p[i] = load_piece<T, false>(from, first + i * 32, d, in);
+    }
   };
   const auto grad = [&](const Row& row, int slot) {
     const float r = row.r;
@@ -269,7 +308,8 @@ norm_grad_rows_kernel(const T* dy, long long dys, Span<T> gin, const T* x, long 
     };
     if (w) sums(std::integral_constant<bool, true>());
     else sums(std::integral_constant<bool, false>());
-    if (ALIGNED) copy(t + S * step, slot);        // the row's values have been used: its place is free
+    if (!ALIGNED) __syncwarp();        // lanes read each other's words
+    copy(t + S * step, slot);          // the row's values have been used: its place is free
     float s1 = warp_sum_f(a2.x + a2.y), s2 = warp_sum_f(b2.x + b2.y);
     if (warps > 1) {
       float2* mine = red[turn] + which * warps;
@@ -282,6 +322,7 @@ norm_grad_rows_kernel(const T* dy, long long dys, Span<T> gin, const T* x, long 
     const float2 m1 = both(-r * (s1 * inv_d)), m2 = both(-r * (s2 * inv_d));
     T* dr = dx + (long long)t * dxs;
     uint4* out = reinterpret_cast<uint4*>(dr) + first;
+    Piece<T> done[NV];
 #pragma unroll
     for (int p = 0; p < NV; ++p) {
 #pragma unroll
@@ -289,9 +330,10 @@ norm_grad_rows_kernel(const T* dy, long long dys, Span<T> gin, const T* x, long 
       if (ALIGNED) {
         if (p < have) out[p * 32] = pack<T>(g[p]).q;
       } else {
-        store_piece<T, false>(dr, first + p * 32, d, pack<T>(g[p]));
+        done[p] = pack<T>(g[p]);
       }
     }
+    if (!ALIGNED) store_pieces(dr, first, d, done);
     t += step;
     turn ^= 1;
   };
@@ -303,36 +345,24 @@ norm_grad_rows_kernel(const T* dy, long long dys, Span<T> gin, const T* x, long 
     }
   };
   statistics(t);
-  if (ALIGNED) {
+  if (ALIGNED)
     for (int i = 0; i < S * 2; ++i)
-      for (int p = have; p < NV; ++p) slots[(i * NV + p) * 32] = make_uint4(0u, 0u, 0u, 0u);     // pieces behind the row stay zero
-    for (int i = 0; i < S; ++i) copy(t + i * step, i);
-    int slot = 0;
-    while (t < rows) {
-      Row row;
-      row.mu = nmu;
-      row.r = nr;
-      copies_wait<S - 1>();
-#pragma unroll
-      for (int p = 0; p < NV; ++p) {
-        row.x[p].q = slots[(slot * 2 * NV + p) * 32];
-        row.g[p].q = slots[(slot * 2 * NV + NV + p) * 32];
-      }
-      statistics(t + step);
-      grad(row, slot);
-      slot = slot + 1 == S ? 0 : slot + 1;
-    }
-    copies_wait<0>();
-  } else {
+      for (int p = have; p < NV; ++p) slots[i * WORDS + p * 32 + lane] = make_uint4(0u, 0u, 0u, 0u);     // pieces behind the row stay zero
+  for (int i = 0; i < S; ++i) copy(t + i * step, i);
+  int slot = 0;
+  while (t < rows) {
     Row row;
-    while (t < rows) {
-      load(t, row);
-      row.mu = nmu;
-      row.r = nr;
-      statistics(t + step);
-      grad(row, 0);
-    }
+    row.mu = nmu;
+    row.r = nr;
+    copies_wait<S - 1>();
+    if (!ALIGNED) __syncwarp();
+    take(x + (long long)t * xs, slots + slot * (2 * WORDS), xin, row.x);
+    take(dy + (long long)t * dys, slots + slot * (2 * WORDS) + WORDS, gin, row.g);
+    statistics(t + step);
+    grad(row, slot);
+    slot = slot + 1 == S ? 0 : slot + 1;
   }
+  copies_wait<0>();
   if (!part) return;
   float* joined = reinterpret_cast<float*>(ring);     // dw then db of the CTA, d each
   float* pw = part + (size_t)blockIdx.x * 2 * d;
@@ -358,8 +388,10 @@ norm_grad_rows_kernel(const T* dy, long long dys, Span<T> gin, const T* x, long 
 }
 
 // Shared memory of that kernel: the rows on their way.  (The sums of the groups that share a CTA, 2 d floats, take less.)
-template <typename T, int NV>
-constexpr size_t norm_grad_smem(int threads) { return (size_t)threads * (norm_grad_ahead<NV>() * 2 * NV * sizeof(uint4)); }
+template <typename T, int NV, bool ALIGNED>
+constexpr size_t norm_grad_smem(int threads) {
+  return (size_t)threads / 32 * (norm_grad_ahead<NV>() * 2 * (NV * 32 + (ALIGNED ? 0 : 1)) * sizeof(uint4));
+}
 
 // Rows wider than the registers take: one CTA per row, the row read again (from L2) for each of its sums.
 template <typename T, typename P>
@@ -491,7 +523,7 @@ int norm_grad_launch(const NormShape& s, int grid, const T* dy, long long dys, c
                      const float* rstd, int rows, int d, const P* w, T* dx, long long dxs, float* part, cudaStream_t stream) {
   return with_pieces<T>(s.nv, [&](auto nv) -> int {
     const auto fn = norm_grad_rows_kernel<T, P, nv(), ALIGNED>;
-    const size_t smem = norm_grad_smem<T, nv()>(s.threads());
+    const size_t smem = norm_grad_smem<T, nv(), ALIGNED>(s.threads());
     KM_CUDA(allow_smem(fn, smem));
     fn<<<grid, dim3(s.group, s.per_cta), smem, stream>>>(
         dy, dys, span_of<T>(dy, dys, rows, d), x, xs, span_of<T>(x, xs, rows, d), mean, rstd, rows, d, 1.f / (float)d, w, dx, dxs,

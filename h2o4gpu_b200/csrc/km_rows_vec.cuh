@@ -191,38 +191,61 @@ __device__ __forceinline__ void store_word(T* row, int c, int d, const Piece<T>&
 template <typename T>
 __device__ __forceinline__ int before_row(const T* row) { return (int)((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(T)); }
 
-// Stores piece i of the row.  Not ALIGNED: all 32 lanes call it with consecutive pieces (lane 0 the first); pieces behind
-// the row's end store nothing.
+// Stores piece i of the row.  Not ALIGNED: all 32 lanes call it with consecutive pieces (store_pieces with one piece a lane).
 template <typename T, bool ALIGNED>
-__device__ __forceinline__ void store_piece(T* row, int i, int d, const Piece<T>& p) {
+__device__ __forceinline__ void store_piece(T* row, int i, int d, const Piece<T>& p);
+
+// Stores NV pieces a lane, piece first + 32 p of the row in lane `first % 32` of its warp: what does not fit a piece's own word goes to the
+// next lane, and from the last lane to the first one's next piece.  All 32 lanes call it; pieces behind the row's end store nothing.
+template <typename T, int NV>
+__device__ __forceinline__ void store_pieces(T* row, int first, int d, const Piece<T> (&p)[NV]) {
   constexpr int V = Piece<T>::V;
-  const int c = i * V;
-  if (ALIGNED) {
-    if (c < d) *reinterpret_cast<uint4*>(row + c) = p.q;
-  } else {
-    const unsigned int off = (unsigned int)(reinterpret_cast<uintptr_t>(row) & 15);   // the same in every lane
-    const int lane = threadIdx.x & 31, m = (int)(off / sizeof(T));
-    // this lane's word: the last m elements of the lane before, then its own first V - m
+  const unsigned int off = (unsigned int)(reinterpret_cast<uintptr_t>(row) & 15);   // the same in every lane
+  const int lane = threadIdx.x & 31, m = (int)(off / sizeof(T));
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int c = (first + i * 32) * V;
+    if (m == 0) {
+      if (c < d) store_word(row, c, d, p[i]);
+      continue;
+    }
+    // this lane's word: the last m elements of the piece before, then its own first V - m
+    const Piece<T>& last = p[i ? i - 1 : 0];
     Piece<T> before;
-    before.w[0] = __shfl_up_sync(0xffffffffu, p.w[0], 1);
-    before.w[1] = __shfl_up_sync(0xffffffffu, p.w[1], 1);
-    before.w[2] = __shfl_up_sync(0xffffffffu, p.w[2], 1);
-    before.w[3] = __shfl_up_sync(0xffffffffu, p.w[3], 1);
-    if ((lane > 0 || m == 0) && c + V - m <= d) {
-      *reinterpret_cast<uint4*>(row + c - m) = m ? shift_words(before.q, p.q, 16 - off) : p.q;
-      if (lane < 31 && c + V < d) return;      // the next lane stores the rest
+#pragma unroll
+    for (int k = 0; k < 4; ++k) before.w[k] = __shfl_sync(0xffffffffu, lane == 31 ? last.w[k] : p[i].w[k], (lane + 31) & 31);
+    if (i == 0 && lane == 0) {      // the piece before is another warp's, or none
 #pragma unroll
       for (int e = 0; e < V; ++e)
-        if (e >= V - m && c + e < d) row[c + e] = p.e[e];
-      return;
-    }
-    // the first lane, or a word that sticks out behind the row: the part of the lane before, then the own
-#pragma unroll
-    for (int e = 0; e < V; ++e) {
-      if (lane > 0 && e >= V - m && c - V + e < d) row[c - V + e] = before.e[e];
-      if (c + e < d && (e < V - m || lane == 31 || c + V >= d)) row[c + e] = p.e[e];
+        if (e < V - m && c + e < d) row[c + e] = p[i].e[e];
+    } else if (c - m < d) {
+      before.q = shift_words(before.q, p[i].q, 16 - off);
+      store_word(row, c - m, d, before);
     }
   }
+  const int c = (first + (NV - 1) * 32) * V;
+  if (lane == 31)
+#pragma unroll
+    for (int e = 0; e < V; ++e)
+      if (e >= V - m && c + e < d) row[c + e] = p[NV - 1].e[e];
+}
+
+template <typename T, bool ALIGNED>
+__device__ __forceinline__ void store_piece(T* row, int i, int d, const Piece<T>& p) {
+  if (ALIGNED) {
+    if (i * Piece<T>::V < d) *reinterpret_cast<uint4*>(row + i * Piece<T>::V) = p.q;
+  } else {
+    const Piece<T> one[1] = {p};
+    store_pieces(row, i, d, one);
+  }
+}
+
+// Whether all words that hold elements of the row lie in the span.
+template <typename T>
+__device__ __forceinline__ bool words_inside(const T* row, int d, const Span<T>& in) {
+  constexpr int V = Piece<T>::V;
+  const T* lo = row - before_row(row);
+  return lo >= in.lo && lo + (before_row(row) + d + V - 1) / V * V <= in.hi;
 }
 
 }  // namespace rows
