@@ -92,11 +92,11 @@ inline int sm_count(int* out) {
 struct ResidentCtas {
   std::atomic<int> known[33] = {};     // by warps
   template <typename F>
-  int get(F fn, int threads, int* out) {
+  int get(F fn, int threads, size_t smem, int* out) {
     std::atomic<int>& k = known[threads / 32];
     *out = k.load(std::memory_order_relaxed);
     if (*out == 0) {
-      KM_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(out, fn, threads, 0));
+      KM_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(out, fn, threads, smem));
       *out = std::max(1, *out);
       k.store(*out, std::memory_order_relaxed);
     }

@@ -38,26 +38,41 @@ __device__ __forceinline__ void load_params(const P* w, int i, int d, bool insid
   }
 }
 
-// Pieces of a row that a lane holds: `have` of them lie in the row, the others are never loaded and stay zero (a load that
+// Pieces of an aligned row that a lane holds: `have` of them lie in the row, the others are never loaded and stay zero (a load that
 // fills in zeros, addresses that are formed for every piece and row cost more instructions than the sums).
-template <typename T, int NV, bool ALIGNED>
-__device__ __forceinline__ void load_pieces(const T* row, int first, int have, int d, const Span<T>& in, Piece<T> (&p)[NV]) {
+template <typename T, int NV>
+__device__ __forceinline__ void load_pieces(const T* row, int first, int have, Piece<T> (&p)[NV]) {
   const uint4* q = reinterpret_cast<const uint4*>(row) + first;
-  if (ALIGNED) {
 #pragma unroll
-    for (int i = 0; i < NV; ++i)
-      if (i < have) p[i].q = q[i * 32];
-  } else if (words_inside(row, d, in)) {      // all rows but a block's first and last
-    constexpr int V = Piece<T>::V;
-    const int m = before_row(row);
-    const uint4* word = reinterpret_cast<const uint4*>(row - m) + first;
+  for (int i = 0; i < NV; ++i)
+    if (i < have) p[i].q = q[i * 32];
+}
+
+// An unaligned row on its way through shared memory: the words that a warp's pieces lie across, 32 NV and one, and the pieces from them.
+// Lanes read each other's words: the warp has to be in step after the copies and before the next ones.  A block's first and last row, whose
+// words may reach beyond it, are loaded when they are taken.
+template <int NV> constexpr int row_words() { return NV * 32 + 1; }
+template <typename T, int NV>
+__device__ __forceinline__ void copy_row(const T* row, int first, int d, const Span<T>& in, uint4* to) {
+  constexpr int V = Piece<T>::V;
+  if (!words_inside(row, d, in)) return;
+  const int lane = threadIdx.x & 31, m = before_row(row), words = (m + d + V - 1) / V;
+  const uint4* q = reinterpret_cast<const uint4*>(row - m) + first;
+#pragma unroll
+  for (int p = 0; p < NV; ++p)
+    if (first + p * 32 < words) copy_async(to + p * 32 + lane, q + p * 32);
+  if (lane == 0 && first + NV * 32 < words) copy_async(to + NV * 32, q + NV * 32);
+}
+template <typename T, int NV>
+__device__ __forceinline__ void take_row(const T* row, int first, int d, const Span<T>& in, const uint4* at, Piece<T> (&p)[NV]) {
+  constexpr int V = Piece<T>::V;
+  if (words_inside(row, d, in)) {
+    const int lane = threadIdx.x & 31, off = before_row(row) * (int)sizeof(T);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int c = (first + i * 32) * V;
-      if (c >= d) continue;
-      const uint4 a = word[i * 32];
-      p[i].q = m && c + V - m < d ? shift_words(a, word[i * 32 + 1], m * (int)sizeof(T)) : shift_words(a, a, m * (int)sizeof(T));
-      clip_piece(p[i], c, d);
+      p[i].q = c < d ? shift_words(at[i * 32 + lane], at[i * 32 + lane + 1], off) : make_uint4(0u, 0u, 0u, 0u);
+      if (c < d) clip_piece(p[i], c, d);
     }
   } else {
 #pragma unroll
@@ -93,6 +108,7 @@ __device__ __forceinline__ void group_sync() {
 // Mean and sum of squared differences from it.  Each warp takes them of its own columns first - its mean, then the differences - and the
 // warps join by  M2 = sum of M2_w + n_w (mean_w - mean)^2:  no cancellation as in E x^2 - (E x)^2, and one barrier instead of two.
 constexpr int kNormMaxThreads = 512;       // a row's group
+constexpr int kNormAhead = 2;              // unaligned rows in shared memory
 template <typename T, typename P, int NV, bool ALIGNED>
 __global__ void __launch_bounds__(kNormMaxThreads)
 norm_rows_kernel(const T* x, long long xs, Span<T> xin, int rows, int d, float inv_d, const P* w, const P* b, float eps, T* y, long long ys,
@@ -109,13 +125,6 @@ norm_rows_kernel(const T* x, long long xs, Span<T> xin, int rows, int d, float i
   const float inv_own = n_own > 0.f ? 1.f / n_own : 0.f, inv_lane = n_lane > 0.f ? 1.f / n_lane : 0.f;
   const int step = gridDim.x * blockDim.y;
   int t = blockIdx.x * blockDim.y + threadIdx.y, turn = 0;
-  // the next row is on its way into one buffer while the other one's sums are formed
-  Piece<T> one[NV], two[NV];
-#pragma unroll
-  for (int p = 0; p < NV; ++p) one[p].q = two[p].q = make_uint4(0u, 0u, 0u, 0u);
-  const auto load = [&](int row, Piece<T>(&p)[NV]) {
-    if (row < rows) load_pieces<T, NV, ALIGNED>(x + (long long)row * xs, first, have, d, xin, p);
-  };
   const auto norm = [&](const Piece<T>(&raw)[NV]) {
     float2 v[NV][H];
 #pragma unroll
@@ -135,7 +144,7 @@ norm_rows_kernel(const T* x, long long xs, Span<T> xin, int rows, int d, float i
 #pragma unroll
       for (int e = 0; e < H; ++e) {
         float2 o = add2(v[p][e], both(-mu));
-        if (!ALIGNED) {
+        if (!ALIGNED && c + V > d) {
           if (c + 2 * e >= d) o.x = 0.f;
           if (c + 2 * e + 1 >= d) o.y = 0.f;
         }
@@ -191,13 +200,44 @@ norm_rows_kernel(const T* x, long long xs, Span<T> xin, int rows, int d, float i
     t += step;
     turn ^= 1;
   };
-  load(t, one);
-  while (t < rows) {
-    load(t + step, two);
-    norm(one);
-    if (t >= rows) break;
-    load(t + step, one);
-    norm(two);
+  if (ALIGNED) {
+    // the next row is on its way into one buffer while the other one's sums are formed
+    Piece<T> one[NV], two[NV];
+#pragma unroll
+    for (int p = 0; p < NV; ++p) one[p].q = two[p].q = make_uint4(0u, 0u, 0u, 0u);
+    const auto load = [&](int row, Piece<T>(&p)[NV]) {
+      if (row < rows) load_pieces(x + (long long)row * xs, first, have, p);
+    };
+    load(t, one);
+    while (t < rows) {
+      load(t + step, two);
+      norm(one);
+      if (t >= rows) break;
+      load(t + step, one);
+      norm(two);
+    }
+  } else {
+    // (a piece can be shifted into place only when it has arrived: in registers the next row would be waited for)
+    constexpr int S = kNormAhead;
+    extern __shared__ uint4 ring[];      // [warp][S][row_words]
+    uint4* slots = ring + (threadIdx.y * warps + in_group / 32) * (S * row_words<NV>());
+    const auto copy = [&](int row, int slot) {
+      if (row < rows) copy_row<T, NV>(x + (long long)row * xs, first, d, xin, slots + slot * row_words<NV>());
+      copies_commit();
+    };
+    for (int i = 0; i < S; ++i) copy(t + i * step, i);
+    int slot = 0;
+    while (t < rows) {
+      Piece<T> raw[NV];
+      copies_wait<S - 1>();
+      __syncwarp();
+      take_row(x + (long long)t * xs, first, d, xin, slots + slot * row_words<NV>(), raw);
+      __syncwarp();
+      copy(t + S * step, slot);
+      norm(raw);
+      slot = slot + 1 == S ? 0 : slot + 1;
+    }
+    copies_wait<0>();
   }
 }
 
@@ -218,7 +258,7 @@ norm_grad_rows_kernel(const T* dy, long long dys, Span<T> gin, const T* x, long 
                       float inv_d, const P* w, T* dx, long long dxs, float* part) {
   constexpr int V = Piece<T>::V, H = V / 2, S = norm_grad_ahead<NV>();
   __shared__ float2 red[2][8];      // used in turn: one half may still be read by slower warps
-  constexpr int WORDS = NV * 32 + (ALIGNED ? 0 : 1);      // of a warp's share of a row; unaligned, its last piece ends one further
+  constexpr int WORDS = ALIGNED ? NV * 32 : row_words<NV>();      // of a warp's share of a row
   extern __shared__ uint4 ring[];   // [warp][S][x, dy][WORDS]; in the end the CTA's sums
   const int group = blockDim.x, per_cta = blockDim.y, which = threadIdx.y, in_group = threadIdx.x, lane = threadIdx.x & 31;
   const int warps = group / 32;
@@ -237,29 +277,21 @@ norm_grad_rows_kernel(const T* dy, long long dys, Span<T> gin, const T* x, long 
     float mu, r;
   };
   uint4* slots = ring + (which * warps + in_group / 32) * (S * 2 * WORDS);
-  // starts the copies of one of a row's two blocks; unaligned: of the words that its pieces lie across
-  const auto copy_block = [&](const T* from, uint4* to) {
+  const auto copy_block = [&](const T* from, const Span<T>& in, uint4* to) {
     if (ALIGNED) {
       const uint4* q = reinterpret_cast<const uint4*>(from) + first;
 #pragma unroll
       for (int p = 0; p < NV; ++p)
         if (p < have) copy_async(to + p * 32 + lane, q + p * 32);
     } else {
-      const int m = before_row(from), words = (m + d + V - 1) / V;
-      const uint4* q = reinterpret_cast<const uint4*>(from - m);
-#pragma unroll
-      for (int p = 0; p < NV; ++p)
-        if (first + p * 32 < words) copy_async(to + p * 32 + lane, q + first + p * 32);
-      if (lane == 0 && first + NV * 32 < words) copy_async(to + NV * 32, q + first + NV * 32);
+      copy_row<T, NV>(from, first, d, in, to);
     }
   };
-  const auto copy = [&](int row, int slot) {
+  const auto copy = [&](int row, int slot) {      // starts the copies of a row
     if (row < rows) {
-      const T* xr = x + (long long)row * xs;
-      const T* gr = dy + (long long)row * dys;
       uint4* to = slots + slot * (2 * WORDS);
-      if (ALIGNED || words_inside(xr, d, xin)) copy_block(xr, to);
-      if (ALIGNED || words_inside(gr, d, gin)) copy_block(gr, to + WORDS);
+      copy_block(x + (long long)row * xs, xin, to);
+      copy_block(dy + (long long)row * dys, gin, to + WORDS);
     }
     copies_commit();
   };
@@ -267,17 +299,8 @@ norm_grad_rows_kernel(const T* dy, long long dys, Span<T> gin, const T* x, long 
     if (ALIGNED) {
 #pragma unroll
       for (int i = 0; i < NV; ++i) p[i].q = at[i * 32 + lane];
-    } else if (words_inside(from, d, in)) {
-      const int off = before_row(from) * (int)sizeof(T);
-#pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        const int c = (first + i * 32) * V;
-        p[i].q = c < d ? shift_words(at[i * 32 + lane], at[i * 32 + lane + 1], off) : make_uint4(0u, 0u, 0u, 0u);
-        if (c < d) clip_piece(p[i], c, d);
-      }
-    } else {      // a block's first or last row
-#pragma unroll
-      for (int i = 0; i < NV; ++i) p[i] = load_piece<T, false>(from, first + i * 32, d, in);
+    } else {
+      take_row(from, first, d, in, at, p);
     }
   };
   const auto grad = [&](const Row& row, int slot) {
@@ -390,7 +413,7 @@ norm_grad_rows_kernel(const T* dy, long long dys, Span<T> gin, const T* x, long 
 // Shared memory of that kernel: the rows on their way.  (The sums of the groups that share a CTA, 2 d floats, take less.)
 template <typename T, int NV, bool ALIGNED>
 constexpr size_t norm_grad_smem(int threads) {
-  return (size_t)threads / 32 * (norm_grad_ahead<NV>() * 2 * (NV * 32 + (ALIGNED ? 0 : 1)) * sizeof(uint4));
+  return (size_t)threads / 32 * (norm_grad_ahead<NV>() * 2 * (ALIGNED ? NV * 32 : row_words<NV>()) * sizeof(uint4));
 }
 
 // Rows wider than the registers take: one CTA per row, the row read again (from L2) for each of its sums.
@@ -509,9 +532,11 @@ int norm_launch(const NormShape& s, int sms, const T* x, long long xs, int rows,
     static ResidentCtas resident;
     const auto fn = norm_rows_kernel<T, P, nv(), ALIGNED>;
     int per_sm = 0;
-    KM_TRY(resident.get(fn, s.threads(), &per_sm));
+    const size_t smem = ALIGNED ? 0 : (size_t)s.threads() / 32 * (kNormAhead * row_words<nv()>() * sizeof(uint4));
+    KM_CUDA(allow_smem(fn, smem));
+    KM_TRY(resident.get(fn, s.threads(), smem, &per_sm));
     const int grid = norm_grid(rows, s, sms, per_sm * s.threads());
-    fn<<<grid, dim3(s.group, s.per_cta), 0, stream>>>(x, xs, span_of<T>(x, xs, rows, d), rows, d, 1.f / (float)d, w, b, eps, y,
+    fn<<<grid, dim3(s.group, s.per_cta), smem, stream>>>(x, xs, span_of<T>(x, xs, rows, d), rows, d, 1.f / (float)d, w, b, eps, y,
                                                                                         ys, mean, rstd);
     KM_CUDA(cudaGetLastError());
     return KM_OK;
