@@ -331,6 +331,28 @@ def test_route_ties_masks_and_infinities(built_lib, dtype):
 
 
 @gpu
+@pytest.mark.parametrize("n", [1, 2, 8, 12])
+@pytest.mark.parametrize("k", [40, 300, 640, 701, 1500, 5000])
+def test_route_of_many_equal_scores(built_lib, k, n):
+    """More scores reach the bound than any list holds, in every kernel: equal ones, masks, infinities, two levels."""
+    R = rows_module(built_lib)
+    for dtype in (torch.float32, torch.bfloat16):
+        s = torch.zeros((70, k), dtype=dtype, device="cuda")
+        s[1:70:9] = torch.finfo(dtype).min
+        s[2:70:9, : k // 2] = 1.0
+        s[3:70:9, ::3] = float("inf")
+        s[4:70:9] = float("nan")
+        s[5:70:9, : k - 3] = float("-inf")
+        s[6:70:9] = torch.arange(k, device="cuda").to(dtype)
+        s[7:70:9] = (torch.arange(k, device="cuda") % 5).to(dtype)
+        s[8:70:9] = -torch.arange(k, device="cuda").to(dtype)
+        for v in (s, s.t().contiguous().t(), torch.cat([s, s], 1)[:, 1:k + 1][:, :k], torch.cat([s, s], 0).t().contiguous().t()[1:]):
+            for over in ("chosen", "all"):
+                check_route(R, v, n, 0.5, over)
+                check_route(R, -v, n, -0.5, over)
+
+
+@gpu
 @pytest.mark.parametrize("over", ["chosen", "all"])
 @pytest.mark.parametrize("dtype", DTYPES, ids=str)
 @pytest.mark.parametrize("shape", ROUTE_SHAPES, ids=str)
@@ -553,6 +575,66 @@ def test_combine_gradient_against_differences(built_lib):
             hi[t][i] += h
             lo[t][i] -= h
             assert abs((loss(*hi) - loss(*lo)) / (2 * h) - float(g[i])) <= 1e-10 + 32 * U * 16
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+def test_rows_at_the_edges_of_their_memory(built_lib, dtype):
+    """Rows that start and end anywhere within 16 bytes, in memory that NaN surrounds: nothing beside them counts, nothing beside the
+    outputs is written."""
+    R = rows_module(built_lib)
+    for d in (1, 2, 3, 5, 7, 8, 9, 15, 17, 31, 33, 255, 257, 1025, 2049):
+        for start in (0, 1, 3, 7):
+            for rows in (1, 2, 5):
+                def at(seed, count):
+                    buf = torch.full((count * d + 32,), float("nan"), dtype=dtype, device="cuda")
+                    view = buf[8 + start:8 + start + count * d].view(count, d)
+                    view.copy_(randn((count, d), seed, dtype))
+                    return view
+                def clean(view):
+                    base = torch.full((view.shape[0] * d + 32,), 9.0, dtype=dtype, device="cuda")
+                    return base, base[8 + (start * 3) % 8:][:view.shape[0] * d].view(view.shape)
+                x, dy = at(180, rows), at(181, rows)
+                f = R.layer_norm(x)
+                y, _, _, tol, _, _ = norm_reference(x, None, None, 1e-5)
+                within(f.y, y, tol)
+                base, o = clean(x)
+                R.layer_norm(x, out=o)
+                assert torch.equal(o, f.y)
+                o.fill_(9.0)
+                assert bool((base == 9.0).all())
+                g = R.layer_norm_grad(dy, x, f.mean, f.rstd)
+                dx, dw, db, tol, tw, tb = norm_grad_reference(dy, x, f.mean, f.rstd, None)
+                within(g.dx, dx, tol)
+                within(g.dweight, dw, tw)
+                n = 2
+                ids = torch.arange(rows * n, device="cuda", dtype=torch.int32).view(rows, n) % 3
+                plan = R.sort_rows(ids, 3)
+                e = at(182, rows * n)
+                w = randn((rows, n), 183)
+                slot = plan.slot.long()
+                base, o = clean(e)
+                R.dispatch(x, plan, out=o)
+                assert torch.equal(o[slot], x[:, None, :].expand(rows, n, d))
+                o.fill_(9.0)
+                assert bool((base == 9.0).all())
+                picked = e.double()[slot] * w.double()[:, :, None]
+                base, o = clean(x)
+                R.combine(e, plan, w, out=o)
+                tol = (n + 1) * U * picked.abs().sum(1)
+                within(o, picked.sum(1), tol + half(dtype) * (picked.sum(1).abs() + tol) + tiny(dtype))
+                o.fill_(9.0)
+                assert bool((base == 9.0).all())
+                drows, dwt = R.combine_grad(dy, e, plan, w)
+                want = dy.double()[:, None, :] * w.double()[:, :, None]
+                within(drows[slot], want, (half(dtype) + 2 * U) * want.abs() + tiny(dtype))
+                dots = e.double()[slot] * dy.double()[:, None, :]
+                within(dwt, dots.sum(2), (d / 32 + 12) * U * dots.abs().sum(2) + 1e-30)
+                if d > 1:
+                    sc = at(184, rows)
+                    got, _ = check_route(R, sc, min(2, d), 1.0, "all")
+                    ds = R.route_grad(torch.ones_like(got.weights), sc, got, 1.0, "all")
+                    assert bool(ds.isfinite().all())
 
 
 @gpu
