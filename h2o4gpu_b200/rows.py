@@ -23,6 +23,7 @@ from .libs import lib_kmeans as _lk
 
 _CODES = {torch.float32: 0, torch.float16: 2, torch.bfloat16: 11}
 _OVER = {"chosen": 0, "all": 1}
+_FEW_ROWS = 256           # rows whose gradient's workspace need not be asked for
 _SORT_ONE_CTA = 2048      # entries below which kmeans_sort_rows needs no workspace
 
 
@@ -215,11 +216,14 @@ def layer_norm_grad(dy, x, mean, rstd, weight=None, params=True):
         return LayerNormGrad(dx, None, None)
     dweight = x.new_empty(cols, dtype=torch.float32)
     dbias = torch.empty_like(dweight)
-    size = ctypes.c_size_t(0)
-    _sizes(_lib.kmeans_layer_norm_grad_workspace, index, rows, cols, ctypes.byref(size))
-    ws = x.new_empty(size.value, dtype=torch.uint8)
+    work = 8 * rows * cols      # a partial sum for every row is always enough
+    if rows > _FEW_ROWS:
+        size = ctypes.c_size_t(0)
+        _sizes(_lib.kmeans_layer_norm_grad_workspace, index, rows, cols, ctypes.byref(size))
+        work = size.value
+    ws = x.new_empty(work, dtype=torch.uint8)
     _call(_lib.kmeans_layer_norm_grad, index, code, dy.data_ptr(), dstride, x.data_ptr(), stride, m, r, rows, cols, w, pcode,
-          dx.data_ptr(), cols, dweight.data_ptr(), dbias.data_ptr(), ws.data_ptr(), size.value)
+          dx.data_ptr(), cols, dweight.data_ptr(), dbias.data_ptr(), ws.data_ptr(), work)
     return LayerNormGrad(dx, dweight, dbias)
 
 
@@ -240,7 +244,7 @@ def _scores(scores):
 
 def _routes(rows, n, like):
     ids = like.new_empty((rows, n), dtype=torch.int32)
-    weights = like.new_empty((rows, n), dtype=torch.float32)
+    weights = torch.empty_like(ids, dtype=torch.float32)
     best = like.new_empty(rows, dtype=torch.float32)
     return Routes(ids, weights, best, torch.empty_like(best))
 

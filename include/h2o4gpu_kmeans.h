@@ -312,8 +312,8 @@ int kmeans_layer_norm(int dtype, const void* x, long long x_stride, size_t rows,
                       const void* bias, int param_dtype, double eps, void* y, long long y_stride, float* mean,
                       float* rstd, void* stream);
 /* Its gradient: dx of the rows' type, dweight and dbias (cols float32 sums over the rows; both or neither).
- * dx may be dy or x.  The workspace (16-byte aligned; not needed without dweight) holds partial sums and is free
- * again when the call's work is done. */
+ * dx may be dy or x.  The workspace (16-byte aligned; not needed without dweight) holds partial sums, never more than
+ * 8 rows cols bytes, and is free again when the call's work is done. */
 int kmeans_layer_norm_grad_workspace(size_t rows, size_t cols, size_t* bytes);
 int kmeans_layer_norm_grad(int dtype, const void* dy, long long dy_stride, const void* x, long long x_stride,
                            const float* mean, const float* rstd, size_t rows, size_t cols, const void* weight,
