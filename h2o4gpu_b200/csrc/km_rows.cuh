@@ -104,6 +104,25 @@ struct ResidentCtas {
   }
 };
 
+// A kernel that is put in place while the one before it on the stream still runs; it has to wait for that one (wait_for_previous) before it
+// touches memory.
+template <typename... P, typename... A>
+int launch_early(void (*fn)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, A... args) {
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  KM_CUDA(cudaLaunchKernelEx(&cfg, fn, static_cast<P>(args)...));
+  return KM_OK;
+}
+__device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 // What a C entry point runs: nothing may leave it but a code.
 template <typename F>
 int guarded(const char* name, F&& f) noexcept {

@@ -486,6 +486,7 @@ norm_grad_sum_kernel(const float* part, int parts, int d, float* dw, float* db) 
   __shared__ float run[32][33];
   const int lane = threadIdx.x, c = blockIdx.x * 32 + lane, per = (parts + 31) / 32;
   float s = 0.f;
+  wait_for_previous();
   if (c < 2 * d)
     for (int p = threadIdx.y * per; p < min(parts, (int)(threadIdx.y + 1) * per); ++p) s += part[(size_t)p * 2 * d + c];
   run[threadIdx.y][lane] = s;

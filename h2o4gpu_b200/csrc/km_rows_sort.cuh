@@ -102,6 +102,7 @@ sort_place_kernel(const int* ids, long long stride, int n, int entries, int k, i
     }
   // every CTA adds up all chunks' counts, so that nothing has to wait for another CTA
   if (part) {
+    wait_for_previous();
     const int words = plan.blocks * k, before = b * k;
 #pragma unroll 4
     for (int i = threadIdx.x; i < words; i += kSortThreads) {

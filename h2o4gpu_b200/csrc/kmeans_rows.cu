@@ -120,8 +120,8 @@ int layer_norm_grad(int dtype, const void* dy, long long dys, const void* x, lon
       }));
   KM_TRY(rc);
   if (part) {
-    norm_grad_sum_kernel<<<(unsigned)((2 * cols + 31) / 32), dim3(32, 32), 0, stream>>>(part, parts, d, dweight, dbias);
-    KM_CUDA(cudaGetLastError());
+    KM_TRY(launch_early(norm_grad_sum_kernel, dim3((unsigned)((2 * cols + 31) / 32)), dim3(32, 32), 0, stream, part, parts, d, dweight,
+                        dbias));
   }
   return KM_OK;
 }
@@ -176,6 +176,9 @@ int sort_rows(const int32_t* ids, long long stride, size_t rows, int n, int k, i
   }
   const size_t smem = (size_t)(plan.warps + 2) * k * sizeof(int);
   KM_CUDA(allow_smem(sort_place_kernel, smem));
+  if (part)
+    return launch_early(sort_place_kernel, dim3(plan.blocks), dim3(kSortThreads), smem, stream, ids, stride, n, entries, k, align, plan, part,
+                        offsets, counts, slot, source, (int)capacity);
   sort_place_kernel<<<plan.blocks, kSortThreads, smem, stream>>>(ids, stride, n, entries, k, align, plan, part, offsets, counts, slot,
                                                                  source, (int)capacity);
   KM_CUDA(cudaGetLastError());
