@@ -90,8 +90,9 @@ dispatch_kernel(const T* x, long long xs, Span<T> xin, int rows, int d, int word
   }
 }
 
-// AT_ONCE entries are on their way together.  Bound by memory: 16,384 x 2048 bfloat16, eight each, take 93 us, 0.99 of the copy rate.  Many warps hide more than many loads a thread do: two rows or two words a thread with twice the
-// registers took 55 and 37 us where this takes 35 (20,011 x 1021 float16, two entries).
+// AT_ONCE entries are on their way together.  Bound by memory: 16,384 x 2048 bfloat16, eight each, take 93 us, 0.99 of the copy rate.
+// Many warps hide more than many loads a thread do: two rows a thread with twice the registers took 55 us where this takes 37 (20,011 x 1021
+// float16, two entries), two words a thread the same 37.
 template <typename T, bool ALIGNED, int AT_ONCE>
 __global__ void __launch_bounds__(kMoveThreads, AT_ONCE > 2 ? 5 : ALIGNED ? 6 : 8)
 combine_kernel(const T* in, long long is, Span<T> iin, int capacity, int d, int words, const int* slot, const float* weights, int rows,
