@@ -154,6 +154,17 @@ def _flat(name, t, index, dtype, shape):
     _refuse(name, t, index, dtype, shape)
 
 
+def _per_entry(name, t, index, dtype, shape):
+    """A tensor of this type and shape on this device in any strides, as one whose elements lie side by side: routes and weights that were
+    sorted from scores lying cluster after cluster lie so too, a gradient may be one number for all.  The caller keeps it until its call is made."""
+    try:
+        if t.dtype is dtype and t.get_device() == index and t.shape == shape:
+            return t if t.is_contiguous() else t.contiguous()
+    except AttributeError:
+        pass
+    _refuse(name, t, index, dtype, shape)
+
+
 def _out(out, like, index, rows, cols, exact=True):
     """The caller's output, or a new one of `like`'s type and device; and its row stride."""
     if out is None:
@@ -267,7 +278,8 @@ def route(scores, n, scale=-1.0, over="chosen"):
 
 def route_grad(dweights, scores, routes, scale=-1.0, over="chosen"):
     """Gradient of the scores, of their type and in their order of dimensions, from that of the weights; `routes`, `scale`
-    and `over` as :func:`route` returned and took them."""
+    and `over` as :func:`route` returned and took them.  Routes and `dweights` may lie in any strides (others than side by side are
+    copied)."""
     rows, k, rs, cs, code, index = _scores(scores)
     flag = _over(over)
     ids, weights, best, total = routes
@@ -275,16 +287,17 @@ def route_grad(dweights, scores, routes, scale=-1.0, over="chosen"):
         raise ValueError("routes.ids must be two-dimensional")
     n, f32 = ids.shape[1], torch.float32
     shape = (rows, n)
-    args = (_flat("routes.ids", ids, index, torch.int32, shape), _flat("routes.weights", weights, index, f32, shape),
-            _flat("routes.best", best, index, f32, (rows,)), _flat("routes.total", total, index, f32, (rows,)))
+    dweights = _per_entry("dweights", dweights, index, f32, shape)
+    routes = (_per_entry("routes.ids", ids, index, torch.int32, shape), _per_entry("routes.weights", weights, index, f32, shape),
+              _per_entry("routes.best", best, index, f32, (rows,)), _per_entry("routes.total", total, index, f32, (rows,)))
     if rs < cs:
         out = scores.new_empty((k, rows)).t()
         drs, dcs = 1, rows
     else:
         out = scores.new_empty((rows, k))
         drs, dcs = k, 1
-    _call(_lib.kmeans_route_grad, index, code, _flat("dweights", dweights, index, f32, shape), scores.data_ptr(), rs, cs,
-          rows, k, n, scale, flag, *args, out.data_ptr(), drs, dcs)
+    _call(_lib.kmeans_route_grad, index, code, dweights.data_ptr(), scores.data_ptr(), rs, cs, rows, k, n, scale, flag,
+          *[t.data_ptr() for t in routes], out.data_ptr(), drs, dcs)
     return out
 
 
@@ -359,13 +372,15 @@ def dispatch_grad(drows, plan, out=None):
 
 
 def combine(rows, plan, weights=None, out=None):
-    """Sum of each row's entries of the sorted `rows` (places, cols), with weights (rows, n) float32 or without; entries
-    that went nowhere add nothing."""
+    """Sum of each row's entries of the sorted `rows` (places, cols), with weights (rows, n) float32 in any strides or without;
+    entries that went nowhere add nothing."""
     have, cols, stride, code, index = _rows("rows", rows)
     slot, _, t, n, places = _plan(plan, index)
     if have < places:
         raise ValueError("rows has %d rows, the plan %d places" % (have, places))
-    w = None if weights is None else _flat("weights", weights, index, torch.float32, (t, n))
+    if weights is not None:
+        weights = _per_entry("weights", weights, index, torch.float32, (t, n))
+    w = None if weights is None else weights.data_ptr()
     y, ystride = _out(out, rows, index, t, cols)
     _call(_lib.kmeans_combine, index, code, rows.data_ptr(), stride, places, cols, slot, w, t, n, y.data_ptr(), ystride)
     return y
@@ -378,9 +393,9 @@ def combine_grad(dy, rows, plan, weights):
     if have < places:
         raise ValueError("rows has %d rows, the plan %d places" % (have, places))
     dstride = _same_rows("dy", dy, rows, index, (t, cols))
-    w = _flat("weights", weights, index, torch.float32, (t, n))
+    weights = _per_entry("weights", weights, index, torch.float32, (t, n))
     drows = rows.new_empty((places, cols))
     dweights = torch.empty_like(weights)
-    _call(_lib.kmeans_combine_grad, index, code, dy.data_ptr(), dstride, rows.data_ptr(), stride, places, cols, slot, source, w, t, n,
-          drows.data_ptr(), cols, dweights.data_ptr())
+    _call(_lib.kmeans_combine_grad, index, code, dy.data_ptr(), dstride, rows.data_ptr(), stride, places, cols, slot, source,
+          weights.data_ptr(), t, n, drows.data_ptr(), cols, dweights.data_ptr())
     return CombineGrad(drows, dweights)
