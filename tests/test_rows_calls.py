@@ -3,11 +3,12 @@ test_rows.py."""
 import os
 import subprocess
 
+import numpy as np
 import pytest
 
 torch = pytest.importorskip("torch")
 
-from test_rows import DTYPES, make_ids, make_scores, randn, rows_module  # noqa: E402
+from test_rows import DTYPES, U, check_route, half, make_ids, make_scores, randn, rows_module, tiny, within  # noqa: E402
 
 gpu = pytest.mark.gpu
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
@@ -111,3 +112,76 @@ def test_combine_grad_of_rows_that_do_not_fill_a_cta(built_lib, dtype):
         apart[:, 0] = dy
         got, want = R.combine_grad(apart[:, 0], e, plan, w), R.combine_grad(dy, e, plan, w)
         assert torch.equal(got.drows, want.drows) and torch.equal(got.dweights, want.dweights)
+
+
+# ---- routing's gradient where masks and limits meet --------------------------------------------------------------------
+
+def check_route_grad(R, s, dw, n, scale, over):
+    """route_grad of what route gives for `s`, against  scale p (g - c)  in float64."""
+    dtype = s.dtype
+    rows, k = s.shape
+    got, ref = check_route(R, s, n, scale, over)
+    ids, w = ref["ids"], got.weights.double().cpu().numpy()
+    g = np.where(ids >= 0, dw.double().cpu().numpy(), 0.0)
+    c = (w * g).sum(1, keepdims=True)
+    dc = (n + 8) * U * np.abs(w * g).sum(1, keepdims=True)
+    G, W = np.zeros((rows, k + 1)), np.zeros((rows, k + 1))
+    np.put_along_axis(G, np.where(ids >= 0, ids, k), g, 1)
+    np.put_along_axis(W, np.where(ids >= 0, ids, k), w, 1)
+    G, W = G[:, :k], W[:, :k]
+    open_ = ref["q"] > -np.inf
+    if over == "chosen":
+        p, drel = W, 0.0
+    else:
+        # exp's argument is off by two roundings of itself, exp by two units in the last place, then a division
+        arg = np.where(open_, ref["a"] * (np.where(open_, ref["q"], 0.0) - ref["base"]), -np.inf)
+        total = got.total.double().cpu().numpy()[:, None]
+        p = np.where(open_ & (total > 0), np.exp(arg) / np.where(total > 0, total, 1.0), 0.0)
+        drel = U * (2 * np.where(open_, np.abs(arg), 0.0) + 6)
+    want = scale * p * (G - c)
+    # beside the result's own roundings, what the smallest exponentials lose below 2^-126
+    tol = abs(scale) * (p * ((drel + 6 * U) * np.abs(G - c) + dc + U * np.abs(G)) + 2.0 ** -126 * (p > 0) * np.abs(G - c)) + 2.0 ** -126
+    tol = tol + half(dtype) * (np.abs(want) + tol) + tiny(dtype)
+    ds = R.route_grad(dw, s, got, scale, over)
+    within(ds, torch.from_numpy(want), torch.from_numpy(tol))
+    assert not bool(ds.cpu()[torch.from_numpy(~open_)].any())        # a cluster that cannot be taken has no gradient
+    return ds
+
+
+def masked_scores(dtype, k=40):
+    """Scores of large quality better: rows that masks of the lowest value, infinities and NaN leave little of."""
+    low, inf, nan = torch.finfo(dtype).min, float("inf"), float("nan")
+    s = torch.zeros((14, k), dtype=dtype, device="cuda")
+    s[1] = low
+    s[2] = -inf
+    s[3] = nan
+    s[4, :k - 2] = -inf
+    s[5, 10:] = low
+    s[6, 7] = s[6, 21] = inf
+    s[7, ::2] = -0.0
+    s[8, 5] = torch.finfo(dtype).max
+    s[9] = torch.arange(k, dtype=torch.float32).to(dtype).cuda()
+    s[10] = nan
+    s[10, k - 1] = low
+    s[11] = -inf                       # one mask by the lowest value, another by -inf, nothing open
+    s[11, 3:9] = low
+    s[12, ::3] = low
+    s[12, 1::3] = -inf
+    s[12, 2::3] = nan
+    s[13] = -inf                       # the lowest value beside infinities of both signs
+    s[13, 4] = inf
+    s[13, 6:11] = low
+    return s
+
+
+@gpu
+@pytest.mark.parametrize("over", ["chosen", "all"])
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("k", [40, 41, 1003])
+def test_route_grad_ties_masks_and_infinities(built_lib, k, dtype, over):
+    R = rows_module(built_lib)
+    s = masked_scores(dtype, k)
+    dw = randn((s.shape[0], 3), 210)
+    for v in (s, by_column(s)):
+        up, down = check_route_grad(R, v, dw, 3, 1.0, over), check_route_grad(R, -v, dw, 3, -1.0, over)
+        assert torch.equal(up, -down)
