@@ -49,6 +49,8 @@ __device__ __forceinline__ float cta_sum(float v, float* red) {
 
 // ---- host side ----------------------------------------------------------------
 constexpr size_t kMaxRows = 0x7fff0000ULL;   // a row or a place is an int, and a grid has room for a few CTAs more
+constexpr size_t kMaxCols = 0x7fff0000ULL;   // a column is an int, and a walk steps behind the last one by what a CTA takes at a time
+constexpr size_t kMaxSumCols = 0x3fff0000ULL;   // the same of the gradients of weight and bias, which lie behind each other
 
 inline cudaStream_t as_stream(void* s) { return static_cast<cudaStream_t>(s); }
 inline int elem_size(int dtype) {
@@ -65,7 +67,7 @@ inline bool aligned(const void* p, size_t to) { return (reinterpret_cast<uintptr
 inline bool block_ok(const void* p, long long stride, size_t rows, size_t cols, int size, bool output) {
   if (!p || !aligned(p, size) || stride < 0) return false;
   if (output && rows > 1 && (unsigned long long)stride < cols) return false;   // rows would overlap
-  return rows <= 0x7fffffffULL && cols <= 0x7fffffffULL && (unsigned long long)stride <= (1ULL << 31);
+  return rows <= kMaxRows && cols <= kMaxCols && (unsigned long long)stride <= (1ULL << 31);
 }
 
 // Whether every row of a block starts on a 16-byte boundary and is whole pieces of 16 bytes long.

@@ -24,6 +24,7 @@ int check_params(const char* name, int dtype, size_t cols, const void* weight, c
   if ((weight && !aligned(weight, size)) || (bias && !aligned(bias, size)))
     KM_FAIL(KM_EINVAL, std::string(name) + ": misaligned weight or bias");
   if (cols < 1) KM_FAIL(KM_EINVAL, std::string(name) + ": cols must be at least 1");
+  if (cols > kMaxCols) KM_FAIL(KM_EINVAL, std::string(name) + ": too many columns");
   return KM_OK;
 }
 
@@ -66,7 +67,7 @@ int norm_grad_parts(size_t rows, size_t cols, int size, int sms) {
 }
 
 int layer_norm_grad_workspace(size_t rows, size_t cols, size_t* bytes) {
-  if (!bytes || cols < 1 || cols > 0x7fffffffULL || rows > kMaxRows) KM_FAIL(KM_EINVAL, "kmeans_layer_norm_grad_workspace: bad argument");
+  if (!bytes || cols < 1 || cols > kMaxSumCols || rows > kMaxRows) KM_FAIL(KM_EINVAL, "kmeans_layer_norm_grad_workspace: bad argument");
   *bytes = 0;
   if (rows == 0) return KM_OK;
   int sms = 0;
@@ -84,7 +85,7 @@ int layer_norm_grad(int dtype, const void* dy, long long dys, const void* x, lon
   KM_TRY(check_params("kmeans_layer_norm_grad", dtype, cols, weight, nullptr, &param_dtype));
   if ((dweight == nullptr) != (dbias == nullptr) || !aligned(dweight, 4) || !aligned(dbias, 4))
     KM_FAIL(KM_EINVAL, "kmeans_layer_norm_grad: dweight and dbias go together");
-  if (rows > kMaxRows || cols > 0x7fffffffULL) KM_FAIL(KM_EINVAL, "kmeans_layer_norm_grad: bad argument");
+  if (rows > kMaxRows || cols > kMaxSumCols) KM_FAIL(KM_EINVAL, "kmeans_layer_norm_grad: too many rows or columns");
   if (rows == 0) {
     if (dweight) {
       KM_CUDA(cudaMemsetAsync(dweight, 0, cols * sizeof(float), stream));
@@ -187,7 +188,7 @@ int sort_rows(const int32_t* ids, long long stride, size_t rows, int n, int k, i
 
 int check_move(const char* name, int dtype, size_t rows, int n, size_t cols, size_t capacity) {
   if (!elem_size(dtype)) KM_FAIL(KM_EINVAL, std::string(name) + ": rows are float32, float16 or bfloat16");
-  if (n < 1 || cols < 1 || cols > 0x7fffffffULL || capacity > kMaxRows || rows > kMaxRows / (size_t)n)
+  if (n < 1 || cols < 1 || cols > kMaxCols || capacity > kMaxRows || rows > kMaxRows / (size_t)n)
     KM_FAIL(KM_EINVAL, std::string(name) + ": bad argument");
   return KM_OK;
 }

@@ -303,7 +303,8 @@ int kmeans_synth_f64(int gpu_id, double* dX, size_t rows, size_t cols, size_t ro
  * when it is stored.  Results do not depend on the schedule: the same call gives the same bits (of route's weights and
  * total, and of dweights, on memory of the same strides and alignment).
  * Arguments are checked before anything is enqueued (KM_EINVAL); rows == 0 is valid and writes what has no rows.
- * Where `rows * n` entries or their places are counted, they are at most 0x7fff0000. */
+ * Where `rows * n` entries or their places are counted, they are at most 0x7fff0000; so are columns (0x3fff0000
+ * in the gradient of layer norm). */
 
 /* Layer norm: mean and 1 / sqrt(variance + eps) of each row, y = (x - mean) * rstd * weight + bias.
  * weight / bias (cols values of param_dtype: float32 or the rows' type) may be NULL, as may mean / rstd (rows

@@ -1,5 +1,6 @@
 """Calls of the row operators (h2o4gpu_b200.rows) that their documentation allows and that need care.  References and tolerances as in
 test_rows.py."""
+import ctypes
 import os
 import subprocess
 
@@ -185,3 +186,29 @@ def test_route_grad_ties_masks_and_infinities(built_lib, k, dtype, over):
     for v in (s, by_column(s)):
         up, down = check_route_grad(R, v, dw, 3, 1.0, over), check_route_grad(R, -v, dw, 3, -1.0, over)
         assert torch.equal(up, -down)
+
+
+# ---- sizes that an int does not hold -----------------------------------------------------------------------------------
+
+def test_c_refuses_more_columns_than_an_int_holds(built_lib):
+    """KM_EINVAL before any device call, for pointers that are never dereferenced."""
+    from h2o4gpu_b200.libs import lib_kmeans
+    lib = lib_kmeans.cdll()
+    p, size = ctypes.c_void_p(4096), ctypes.c_size_t()
+    most, most_grad = 0x7fff0000, 0x3fff0000
+
+    def norm(cols):
+        return lib.kmeans_layer_norm(2, p, cols, 1, cols, None, None, 0, 1e-5, p, cols, p, p, None)
+
+    def norm_grad(cols):
+        return lib.kmeans_layer_norm_grad(2, p, cols, p, cols, p, p, 1, cols, None, 0, p, cols, p, p, p, 1 << 50, None)
+
+    def moves(cols):
+        return [lib.kmeans_dispatch(2, p, cols, 1, cols, 1, p, p, 1, p, cols, None),
+                lib.kmeans_combine(2, p, cols, 1, cols, p, p, 1, 1, p, cols, None),
+                lib.kmeans_combine_grad(2, p, cols, p, cols, 1, cols, p, p, p, 1, 1, p, cols, p, None)]
+
+    for cols in (most + 1, 0x7fffffff, 1 << 31, (1 << 32) + 8):
+        assert norm(cols) == -1 and norm_grad(cols) == -1 and moves(cols) == [-1, -1, -1], cols
+    for cols in (most_grad + 1, 1 << 30, 1_200_000_000):
+        assert norm_grad(cols) == -1 and lib.kmeans_layer_norm_grad_workspace(1, cols, ctypes.byref(size)) == -1, cols
