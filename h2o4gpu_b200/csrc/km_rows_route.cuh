@@ -618,7 +618,9 @@ route_grad_warp_kernel(const float* dweights, const T* s, long long rs, Span<T> 
     sum = total[t];
   }
   const bool taken = id >= 0 && id < k;
-  const float c = warp_sum_f(taken ? w * g : 0.f), f = OVER_ALL && sum > 0.f ? -scale * c / sum : 0.f;
+  const float c = warp_sum_f(taken ? w * g : 0.f);
+  float f = OVER_ALL && sum > 0.f ? -scale * c / sum : 0.f;
+  const bool far = !(fabsf(f) <= 3.402823466e38f);
   // perhaps an infinitely good score, which counts as this; an infinitely bad one then lies so far off that its difference is infinite again
   // (where the best score is the lowest number, closed clusters have to stay infinite)
   const bool huge = b == copysignf(3.402823466e38f, scale);
@@ -648,6 +650,14 @@ route_grad_warp_kernel(const float* dweights, const T* s, long long rs, Span<T> 
     store_piece<T, ALIGNED>(dr, i, k, p);
   }
   __syncwarp();
+  if (far) {      // the scale is applied last, so that 0 times it stays 0
+    f = -c / sum;
+    for (int e = lane; e < k; e += 32) {
+      const float o = to_f(sr[e]), x = scale * ((huge ? route_finite(o) : o) - b);
+      dr[e] = from_f<T>(scale * (f * expf(fmaxf(x, -INFINITY))));
+    }
+    __syncwarp();
+  }
   if (taken) dr[id] = from_f<T>(scale * w * (g - c));
 }
 
@@ -667,7 +677,12 @@ route_grad_lane_kernel(const float* dweights, const T* s, long long rs, long lon
     if (id >= 0 && id < k) c = fmaf(weights[(long long)t * n + j], dweights[(long long)t * n + j], c);
   }
   const float sign = scale > 0.f ? 1.f : -1.f, a = fabsf(scale);
-  const float sum = over_all ? total[t] : 0.f, q0 = over_all ? sign * best[t] : 0.f, f = sum > 0.f ? -scale * c / sum : 0.f;
+  const float sum = over_all ? total[t] : 0.f, q0 = over_all ? sign * best[t] : 0.f;
+  float f = sum > 0.f ? -scale * c / sum : 0.f, last = 1.f;
+  if (!(fabsf(f) <= 3.402823466e38f)) {      // the scale is then applied last: 0 times it stays 0
+    f = -c / sum;
+    last = scale;
+  }
   const T* sr = s + t * rs;
   T* dr = ds + t * drs;
 #pragma unroll 8
@@ -675,7 +690,7 @@ route_grad_lane_kernel(const float* dweights, const T* s, long long rs, long lon
     float v = 0.f;
     if (over_all) {
       const float q = route_value(sr[e * cs], sign);
-      if (q > -INFINITY) v = f * expf(a * (q - q0));
+      if (q > -INFINITY) v = last * (f * expf(a * (q - q0)));
     }
     dr[e * dcs] = from_f<T>(v);
   }

@@ -9,7 +9,7 @@ import pytest
 
 torch = pytest.importorskip("torch")
 
-from test_rows import DTYPES, U, check_route, half, make_ids, make_scores, randn, rows_module, tiny, within  # noqa: E402
+from test_rows import DTYPES, HUGE, U, check_route, half, make_ids, make_scores, randn, rows_module, tiny, within  # noqa: E402
 
 gpu = pytest.mark.gpu
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
@@ -186,6 +186,22 @@ def test_route_grad_ties_masks_and_infinities(built_lib, k, dtype, over):
     for v in (s, by_column(s)):
         up, down = check_route_grad(R, v, dw, 3, 1.0, over), check_route_grad(R, -v, dw, 3, -1.0, over)
         assert torch.equal(up, -down)
+
+
+@gpu
+@pytest.mark.parametrize("over", ["chosen", "all"])
+@pytest.mark.parametrize("k", [40, 41, 200])
+def test_route_grad_with_the_largest_scales(built_lib, k, over):
+    """The scale times the weights' gradient is beyond float32, the gradient of clusters without weight is zero all the same."""
+    R = rows_module(built_lib)
+    s = make_scores(20, k, torch.float32, 211, masked=False)
+    s[:, 7] = s[:, 3]
+    s[1::2, 5:30:3] = float("-inf")
+    for shift in (0.0, 3.0):
+        dw = randn((20, 4), 212, scale=2.0, shift=shift)
+        for scale in (HUGE / 2, -HUGE / 2, 2.0 ** -126):
+            for v in (s, by_column(s)):
+                check_route_grad(R, v if scale > 0 else -v, dw, 4, scale, over)
 
 
 # ---- sizes that an int does not hold -----------------------------------------------------------------------------------
