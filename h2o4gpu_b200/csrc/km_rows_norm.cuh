@@ -307,7 +307,7 @@ norm_grad_rows_kernel(const T* dy, long long dys, Span<T> gin, const T* x, long 
   };
   const auto grad = [&](const Row& row, int slot) {
     const float r = row.r;
-    const float2 rr = both(r), off = both(-row.mu * r);      // xh = x r - mu r: this rounding is no larger than the stored mean's
+    const float2 rr = both(r), off = both(-row.mu);      // (x - mu is exact or nearly so for rows far from zero, x r - mu r would not be)
     float2 xh[NV][H], g[NV][H];
 #pragma unroll
     for (int p = 0; p < NV; ++p) {
@@ -322,7 +322,7 @@ norm_grad_rows_kernel(const T* dy, long long dys, Span<T> gin, const T* x, long 
         if (with_w()) load_params<P, H, ALIGNED>(w, first + p * 32, d, p < have, w_words, 1.f, wf);
 #pragma unroll
         for (int e = 0; e < H; ++e) {
-          xh[p][e] = fma2(xh[p][e], rr, off);     // behind the row's end g is zero
+          xh[p][e] = mul2(add2(xh[p][e], off), rr);     // behind the row's end g is zero
           aw[p][e] = fma2(g[p][e], xh[p][e], aw[p][e]);
           ab[p][e] = add2(ab[p][e], g[p][e]);
           if (with_w()) g[p][e] = mul2(g[p][e], wf[e]);

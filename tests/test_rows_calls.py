@@ -115,6 +115,35 @@ def test_combine_grad_of_rows_that_do_not_fill_a_cta(built_lib, dtype):
         assert torch.equal(got.drows, want.drows) and torch.equal(got.dweights, want.dweights)
 
 
+# ---- layer norm's gradient of rows far from zero -----------------------------------------------------------------------
+
+@gpu
+@pytest.mark.parametrize("shape", [(5, 64), (5, 500), (6, 784), (5, 1021), (3, 4096), (4, 8100), (3, 9000)], ids=str)
+def test_layer_norm_grad_far_from_zero(built_lib, shape):
+    """Rows whose mean is thousands of deviations away: x - mean loses nothing there (the difference of two near numbers is exact), so the
+    gradient is off by the roundings of the small numbers alone."""
+    R = rows_module(built_lib)
+    rows, d = shape
+    x = randn(shape, 220, torch.float32, 1.0, 5000.0)
+    x[1] -= 9000.0
+    w, dy = randn(d, 221, scale=0.1, shift=1.0), randn(shape, 222)
+    f = R.layer_norm(x)
+    for weight in (w, None):
+        got = R.layer_norm_grad(dy, x, f.mean, f.rstd, weight)
+        r = f.rstd.double()[:, None]
+        xh = (x.double() - f.mean.double()[:, None]) * r
+        dyd = dy.double()
+        g = dyd if weight is None else dyd * w.double()
+        m1, m2 = g.mean(1, keepdim=True), (g * xh).mean(1, keepdim=True)
+        dx = r * (g - m1 - xh * m2)
+        # xh: a difference and a product; g: a product; each mean: its additions and two products; the result: five operations
+        depth = d / 32 + 12
+        tol = U * r * (8 * g.abs() + (depth + 8) * g.abs().mean(1, keepdim=True) + (depth + 14) * xh.abs() * (g * xh).abs().mean(1, keepdim=True))
+        within(got.dx, dx, tol + U * dx.abs())
+        within(got.dweight, (dyd * xh).sum(0), U * (rows + 18) * (dyd * xh).abs().sum(0))
+        within(got.dbias, dyd.sum(0), U * (rows + 4) * dyd.abs().sum(0))
+
+
 # ---- routing's gradient where masks and limits meet --------------------------------------------------------------------
 
 def check_route_grad(R, s, dw, n, scale, over):
