@@ -25,6 +25,8 @@ _CODES = {torch.float32: 0, torch.float16: 2, torch.bfloat16: 11}
 _OVER = {"chosen": 0, "all": 1}
 _FEW_ROWS = 256           # rows whose gradient's workspace need not be asked for
 _SORT_ONE_CTA = 2048      # entries below which kmeans_sort_rows needs no workspace
+_SORT_KNOWN = 16384       # k and align up to which the places of so few entries need not be asked for
+_INT = 0x7fffffff         # ctypes would cut what is more down to a C int without a word
 
 
 class LayerNorm(NamedTuple):
@@ -250,6 +252,8 @@ def _scores(scores):
         _refuse("scores", scores)
     if index < 0:
         _refuse("scores", scores)
+    if k > _INT:
+        raise ValueError("scores of %d clusters are too many" % k)
     return rows, k, rs, cs, code, index
 
 
@@ -269,6 +273,8 @@ def route(scores, n, scale=-1.0, over="chosen"):
     bad scores are never chosen."""
     rows, k, rs, cs, code, index = _scores(scores)
     flag = _over(over)
+    if not 0 < n <= k:
+        raise ValueError("a row takes 1 to %d clusters, not %s" % (k, n))
     out = _routes(rows, n, scores)
     ids, weights, best, total = out
     _call(_lib.kmeans_route, index, code, scores.data_ptr(), rs, cs, rows, k, n, scale, flag, ids.data_ptr(),
@@ -286,6 +292,8 @@ def route_grad(dweights, scores, routes, scale=-1.0, over="chosen"):
     if ids.dim() != 2:
         raise ValueError("routes.ids must be two-dimensional")
     n, f32 = ids.shape[1], torch.float32
+    if n > k:
+        raise ValueError("routes of %d clusters a row, scores of %d" % (n, k))
     shape = (rows, n)
     dweights = _per_entry("dweights", dweights, index, f32, shape)
     routes = (_per_entry("routes.ids", ids, index, torch.int32, shape), _per_entry("routes.weights", weights, index, f32, shape),
@@ -304,6 +312,8 @@ def route_grad(dweights, scores, routes, scale=-1.0, over="chosen"):
 def nearest(handle, n, scale=-1.0, over="chosen", local=0):
     """:func:`route` on the distances of a ``ResidentKMeans`` handle's shard `local` to its centroids, which never leave the
     device: the n nearest clusters of every row.  float32 handles."""
+    if n > _INT:
+        raise ValueError("%d clusters a row are too many" % n)
     dev = torch.device("cuda", handle.shard_device(local))
     out = _routes(handle.shard_rows(local), n, torch.empty(0, device=dev))
     torch.cuda.current_stream(dev).synchronize()      # the handle's stream is another one
@@ -326,9 +336,11 @@ def sort_rows(ids, k, align=1):
     stride, inner = ids.stride()
     if inner != 1 and n > 1:
         raise ValueError("ids: the elements of a row must lie side by side")
+    if not 0 < k <= _INT or not 0 < align <= _INT or n > _INT:
+        raise ValueError("k, align and the entries of a row are 1 to %d, not %s, %s and %d" % (_INT, k, align, n))
     index, entries = ids.get_device(), rows * n
     places, work = entries + min(k, entries) * (align - 1), 0
-    if entries >= _SORT_ONE_CTA:
+    if entries >= _SORT_ONE_CTA or k > _SORT_KNOWN or align > _SORT_KNOWN:
         capacity, size = ctypes.c_size_t(0), ctypes.c_size_t(0)
         _sizes(_lib.kmeans_sort_rows_sizes, index, rows, n, k, align, ctypes.byref(capacity), ctypes.byref(size))
         places, work = capacity.value, size.value
@@ -350,6 +362,8 @@ def _plan(plan, index):
         places, = source.shape
     except ValueError:
         raise ValueError("plan.slot must be two-dimensional and plan.source one-dimensional") from None
+    if n > _INT:
+        raise ValueError("a plan of %d entries a row has too many" % n)
     return (_flat("plan.slot", slot, index, torch.int32, slot.shape), _flat("plan.source", source, index, torch.int32, source.shape),
             rows, n, places)
 

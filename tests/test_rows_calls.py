@@ -257,3 +257,34 @@ def test_c_refuses_more_columns_than_an_int_holds(built_lib):
         assert norm(cols) == -1 and norm_grad(cols) == -1 and moves(cols) == [-1, -1, -1], cols
     for cols in (most_grad + 1, 1 << 30, 1_200_000_000):
         assert norm_grad(cols) == -1 and lib.kmeans_layer_norm_grad_workspace(1, cols, ctypes.byref(size)) == -1, cols
+
+
+@gpu
+def test_python_refuses_sizes_that_a_c_int_cuts(built_lib):
+    """2^32 + 8 clusters would arrive as 8; and what is refused allocates nothing first."""
+    R = rows_module(built_lib)
+    from h2o4gpu_b200 import ResidentKMeans
+    x = randn((6, 8), 230)
+    wide = torch.zeros((1, 1), device="cuda").expand(1, (1 << 32) + 8)
+    ids = torch.zeros((6, 2), dtype=torch.int32, device="cuda")
+    r = R.route(x, 2)
+    one = R.Routes(r.ids[:1], r.weights[:1], r.best[:1], r.total[:1])
+    h = ResidentKMeans()
+    bad = [lambda: R.route(wide, 2), lambda: R.route(x, (1 << 32) + 2), lambda: R.route(x, 1 << 20),
+           lambda: R.route_grad(one.weights, wide, one), lambda: R.nearest(h, (1 << 32) + 1),
+           lambda: R.sort_rows(ids, (1 << 32) + 3), lambda: R.sort_rows(ids, 3, (1 << 32) + 1), lambda: R.sort_rows(ids, 1 << 30),
+           lambda: R.sort_rows(ids, 3, 1 << 30), lambda: R.sort_rows(ids, -3), lambda: R.sort_rows(ids, 3, -1)]
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    for i, call in enumerate(bad):
+        with pytest.raises((ValueError, RuntimeError)):
+            call()
+            pytest.fail("call %d was not refused" % i)
+    assert torch.cuda.max_memory_allocated() - before < 1 << 20
+    h.close()
+    # the largest of what is taken
+    plan = R.sort_rows(ids, 16384, 16384)
+    assert plan.offsets[1:].tolist() == [16384] * 16384 and plan.slot.view(-1).tolist() == list(range(12))
+    plan = R.sort_rows(ids[:1], 3, 1 << 20)
+    assert plan.offsets.tolist() == [0, 1 << 20, 1 << 20, 1 << 20] and plan.source[:2].tolist() == [0, 1]
