@@ -505,6 +505,13 @@ int Engine<T>::attach_device(int local, const T* dX, size_t rows, size_t cols, s
   if (d != 0 && d != (int)cols && local != 0) KM_FAIL(KM_EINVAL, "kmeans_attach_device: shards disagree on cols");
   Shard<T>& s = shards[local];
   DevGuard g(s.dev);
+  if (s.labels_cap < rows) {      // first, so that a handle that gets no memory keeps what it had
+    int* labels = nullptr;
+    KM_CUDA(km_malloc(&labels, rows * sizeof(int)));
+    km_free(s.labels);
+    s.labels = labels;
+    s.labels_cap = rows;
+  }
   if (s.X_owned && s.X_owned != dX) { km_free(s.X_owned); s.X_owned = nullptr; }
   s.X = dX;
   s.rows = rows;
@@ -523,12 +530,6 @@ int Engine<T>::attach_device(int local, const T* dX, size_t rows, size_t cols, s
   if ((int)cols != d) have_centroids = false;
   d = (int)cols;
   n_total = ntot;
-  if (s.labels_cap < rows) {
-    km_free(s.labels);
-    s.labels = nullptr;
-    KM_CUDA(km_malloc(&s.labels, rows * sizeof(int)));
-    s.labels_cap = rows;
-  }
   KM_CUDA(cudaMemsetAsync(s.labels, 0xff, rows * sizeof(int), s.stream));
   KM_CUDA(cudaMemsetAsync(&s.st->full_rows, 0, 2 * sizeof(unsigned int), s.stream));   // and pad_ready
   return KM_OK;
@@ -838,6 +839,8 @@ int Engine<T>::upload_host_typed(const void* Xv, int src_dtype, size_t rows, siz
     const size_t r = per + (i < extra ? 1 : 0);
     if (r == 0) { upload_wait(); KM_FAIL(KM_EINVAL, "kmeans_upload_host: fewer rows than devices"); }
     DevGuard gd(s.dev);
+    s.X = nullptr;      // until the new matrix is attached the shard has none
+    s.rows = 0;
     km_free(s.X_owned);
     s.X_owned = nullptr;
     km_free(s.raw);
@@ -880,7 +883,8 @@ int Engine<T>::upload_host_typed(const void* Xv, int src_dtype, size_t rows, siz
       km_free(s.raw);
       s.raw = nullptr;
     }
-    KM_TRY(attach_device((int)i, s.X_owned, r, cols, rows));
+    const int rc = attach_device((int)i, s.X_owned, r, cols, rows);
+    if (rc != KM_OK) { upload_wait(); return rc; }
     s.row0 = off;
     off += r;
   }

@@ -553,6 +553,7 @@ template <typename T>
 template <typename Sink>
 int Engine<T>::distance_blocks(int local, const Sink& sink) {
   Shard<T>& s = shards[local];
+  if (!s.X) KM_FAIL(KM_ESTATE, "no data attached to the handle");
   // max|x| (the tensor-core kernel's operand scale) is known after the data check; with several
   // processes that check is a collective and is left to the fit
   if (world_size == (int)shards.size()) KM_TRY(check_data());

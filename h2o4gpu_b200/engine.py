@@ -81,6 +81,7 @@ class ResidentKMeans(object):
             order = 'c' if (X.flags.f_contiguous and not X.flags.c_contiguous) else 'r'
         X = np.ascontiguousarray(X) if order == 'r' else np.asfortranarray(X)
         rows, cols = X.shape
+        self._rows = [0] * self.n_local           # what a failed upload leaves
         _lk.check(self._lib.kmeans_upload_host_typed(self._h, X.ctypes.data_as(ctypes.c_void_p),
                                                      DTYPE_CODES[X.dtype], rows, cols, order.encode()))
         per, extra = divmod(rows, self.n_local)   # the library's balanced contiguous split
@@ -127,7 +128,7 @@ class ResidentKMeans(object):
         return out
 
     def labels(self, local=0):
-        out = np.empty(self._rows[local], dtype=np.int32)
+        out = np.empty(self.shard_rows(local), dtype=np.int32)
         _lk.check(self._lib.kmeans_get_labels(self._h, local, out.ctypes.data_as(ctypes.c_void_p)))
         return out
 
@@ -141,13 +142,15 @@ class ResidentKMeans(object):
 
     def transform(self, local=0):
         """Squared distances of one shard, (rows, k), Fortran-ordered."""
-        rows = self._rows[local]
+        rows = self.shard_rows(local)
         out = np.empty(rows * self.k, dtype=self.dtype)
         _lk.check(self._lib.kmeans_transform_resident(self._h, local, out.ctypes.data_as(ctypes.c_void_p), rows))
         return out.reshape((rows, self.k), order='F')
 
     def shard_rows(self, local=0):
-        """Rows of one shard."""
+        """Rows of one shard; raises if it has no data (a failed upload leaves none)."""
+        if not self._rows[local]:
+            raise RuntimeError("no data attached to shard %d of the handle" % local)
         return self._rows[local]
 
     def shard_device(self, local=0):

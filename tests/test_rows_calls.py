@@ -288,3 +288,41 @@ def test_python_refuses_sizes_that_a_c_int_cuts(built_lib):
     assert plan.offsets[1:].tolist() == [16384] * 16384 and plan.slot.view(-1).tolist() == list(range(12))
     plan = R.sort_rows(ids[:1], 3, 1 << 20)
     assert plan.offsets.tolist() == [0, 1 << 20, 1 << 20, 1 << 20] and plan.source[:2].tolist() == [0, 1]
+
+
+# ---- a handle that got no memory ---------------------------------------------------------------------------------------
+
+@gpu
+def test_nearest_after_a_failed_attach_or_upload(built_lib):
+    """The outputs have the rows that the engine works on: a failed attach leaves the old matrix, a failed upload none."""
+    from h2o4gpu_b200 import ResidentKMeans
+    from h2o4gpu_b200.libs import lib_kmeans
+    R = rows_module(built_lib)
+    lib = lib_kmeans.cdll()
+    few, many = randn((300, 16), 240), randn((200_000, 16), 241)
+    h = ResidentKMeans()
+    h.attach_device(0, few.data_ptr(), 300, 16)
+    h.set_centroids(few[:7].cpu().numpy())
+    h.assign()
+    want, labels = R.nearest(h, 3), h.labels()
+
+    def fails(call):
+        lib.kmeans_selftest_alloc_limit(1000)
+        try:
+            with pytest.raises(RuntimeError):
+                call()
+        finally:
+            lib.kmeans_selftest_alloc_limit(-1)
+
+    fails(lambda: h.attach_device(0, many.data_ptr(), 200_000, 16))
+    assert all(torch.equal(a, b) for a, b in zip(R.nearest(h, 3), want)) and np.array_equal(h.labels(), labels)
+    fails(lambda: h.upload(many.cpu().numpy()))
+    for call in (lambda: R.nearest(h, 3), h.transform, h.labels, lambda: h.fit(few[:7].cpu().numpy(), 2), h.assign):
+        with pytest.raises(RuntimeError, match="no data"):
+            call()
+    h.upload(few.cpu().numpy())
+    h.set_centroids(few[:7].cpu().numpy())
+    assert all(torch.equal(a, b) for a, b in zip(R.nearest(h, 3), want))
+    h.attach_device(0, many.data_ptr(), 200_000, 16)
+    assert R.nearest(h, 3).ids.shape == (200_000, 3)
+    h.close()
