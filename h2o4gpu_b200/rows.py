@@ -282,15 +282,33 @@ def route(scores, n, scale=-1.0, over="chosen"):
     return out
 
 
-def route_grad(dweights, scores, routes, scale=-1.0, over="chosen"):
+def _no_scores(ids, k, dtype, over):
+    """What :func:`_scores` gives, of scores that are not at hand: as if they lay row after row."""
+    if over != "chosen":
+        raise ValueError("weights over all clusters: their gradient needs the scores")
+    if dtype not in _CODES:
+        raise ValueError("dtype must be float32, float16 or bfloat16, not %s" % dtype)
+    if not isinstance(ids, torch.Tensor) or not ids.is_cuda or ids.dim() != 2:
+        _refuse("routes.ids", ids, None, torch.int32)
+    if k is None or not 0 < k <= _INT:
+        raise ValueError("without scores, k is the number of clusters, not %s" % k)
+    return ids.shape[0], k, k, 1, _CODES[dtype], ids.get_device()
+
+
+def route_grad(dweights, scores, routes, scale=-1.0, over="chosen", k=None, dtype=torch.float32):
     """Gradient of the scores, of their type and in their order of dimensions, from that of the weights; `routes`, `scale`
     and `over` as :func:`route` returned and took them.  Routes and `dweights` may lie in any strides (others than side by side are
-    copied)."""
-    rows, k, rs, cs, code, index = _scores(scores)
+    copied).  Over the chosen clusters no score is read: `scores` may be None (behind :func:`nearest`, whose distances nobody
+    has), the gradient then is (rows, `k`) of `dtype`, row after row.  With scores, `k` and `dtype` are theirs."""
+    ids, weights, best, total = (None,) * 4 if routes is None else routes
+    if scores is None:
+        rows, k, rs, cs, code, index = _no_scores(ids, k, dtype, over)
+    else:
+        rows, k, rs, cs, code, index = _scores(scores)
+        dtype = scores.dtype
     flag = _over(over)
-    ids, weights, best, total = routes
-    if ids.dim() != 2:
-        raise ValueError("routes.ids must be two-dimensional")
+    if not isinstance(ids, torch.Tensor) or ids.dim() != 2:
+        raise ValueError("routes.ids must be a two-dimensional tensor")
     n, f32 = ids.shape[1], torch.float32
     if n > k:
         raise ValueError("routes of %d clusters a row, scores of %d" % (n, k))
@@ -299,13 +317,13 @@ def route_grad(dweights, scores, routes, scale=-1.0, over="chosen"):
     routes = (_per_entry("routes.ids", ids, index, torch.int32, shape), _per_entry("routes.weights", weights, index, f32, shape),
               _per_entry("routes.best", best, index, f32, (rows,)), _per_entry("routes.total", total, index, f32, (rows,)))
     if rs < cs:
-        out = scores.new_empty((k, rows)).t()
+        out = dweights.new_empty((k, rows), dtype=dtype).t()
         drs, dcs = 1, rows
     else:
-        out = scores.new_empty((rows, k))
+        out = dweights.new_empty((rows, k), dtype=dtype)
         drs, dcs = k, 1
-    _call(_lib.kmeans_route_grad, index, code, dweights.data_ptr(), scores.data_ptr(), rs, cs, rows, k, n, scale, flag,
-          *[t.data_ptr() for t in routes], out.data_ptr(), drs, dcs)
+    _call(_lib.kmeans_route_grad, index, code, dweights.data_ptr(), None if scores is None else scores.data_ptr(), rs, cs, rows, k, n,
+          scale, flag, *[t.data_ptr() for t in routes], out.data_ptr(), drs, dcs)
     return out
 
 

@@ -144,6 +144,49 @@ def test_layer_norm_grad_far_from_zero(built_lib, shape):
         within(got.dbias, dyd.sum(0), U * (rows + 4) * dyd.abs().sum(0))
 
 
+# ---- backward from the engine's own routes, whose scores nobody has ----------------------------------------------------
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+def test_route_grad_without_scores(built_lib, dtype):
+    """Over the chosen no score is read: the same gradient without them, bit by bit."""
+    R = rows_module(built_lib)
+    for rows, k, n in ((70, 33, 5), (1, 8, 2), (300, 100, 4), (50, 1000, 32)):
+        s, dw = make_scores(rows, k, dtype, 250), randn((rows, n), 251)
+        r = R.route(s, n, 0.5)
+        assert torch.equal(R.route_grad(dw, None, r, 0.5, k=k, dtype=dtype), R.route_grad(dw, s, r, 0.5))
+    for bad in (lambda: R.route_grad(dw, None, r, 0.5), lambda: R.route_grad(dw, None, r, 0.5, "all", k=k),
+                lambda: R.route_grad(dw, None, r, 0.5, k=n - 1), lambda: R.route_grad(dw, None, r, 0.5, k=k, dtype=torch.float64),
+                lambda: R.route_grad(dw[:3], None, r, 0.5, k=k), lambda: R.route_grad(dw, None, None, 0.5, k=k),
+                lambda: R.route_grad(dw, s, None, 0.5)):
+        with pytest.raises(ValueError):
+            bad()
+
+
+@gpu
+def test_route_grad_behind_nearest(built_lib):
+    """A handle's nearest clusters, and the gradient of its distances from that of their weights."""
+    from h2o4gpu_b200 import ResidentKMeans
+    R = rows_module(built_lib)
+    rows, d, k, n = 900, 24, 9, 3
+    X = randn((rows, d), 252)
+    h = ResidentKMeans()
+    h.attach_device(0, X.data_ptr(), rows, d)
+    h.set_centroids(X[:k].cpu().numpy())
+    r = R.nearest(h, n, -0.1)
+    D = torch.from_numpy(h.transform()).cuda()
+    h.close()
+    dw = randn((rows, n), 253)
+    got = R.route_grad(dw, None, r, -0.1, k=k)
+    assert got.shape == (rows, k) and got.dtype == torch.float32
+    # D lies cluster after cluster, where another kernel adds up c in another order: each of the two is off by at most n + 8 roundings of
+    # sum |w g|, two of |g| (the difference), and four of the result
+    w, g = r.weights.double(), dw.double()
+    size = 0.1 * w * ((n + 12) * (w * g).abs().sum(1, keepdim=True) + 6 * g.abs())
+    tol = torch.zeros((rows, k), dtype=torch.float64, device="cuda").scatter_(1, r.ids.long(), 2 * U * size)
+    within(got, R.route_grad(dw, D, r, -0.1), tol)
+
+
 # ---- routing's gradient where masks and limits meet --------------------------------------------------------------------
 
 def check_route_grad(R, s, dw, n, scale, over):
@@ -326,3 +369,12 @@ def test_nearest_after_a_failed_attach_or_upload(built_lib):
     h.attach_device(0, many.data_ptr(), 200_000, 16)
     assert R.nearest(h, 3).ids.shape == (200_000, 3)
     h.close()
+
+
+def test_route_grad_without_scores_refuses_what_is_not_on_a_gpu(built_lib):
+    R = rows_module(built_lib)
+    ids = torch.zeros((4, 2), dtype=torch.int32)
+    with pytest.raises(ValueError, match="must be a CUDA tensor"):
+        R.route_grad(ids.float(), None, R.Routes(ids, ids.float(), ids[:, 0].float(), ids[:, 0].float()), k=3)
+    with pytest.raises(ValueError, match="needs the scores"):
+        R.route_grad(ids.float(), None, R.Routes(ids, ids.float(), ids[:, 0].float(), ids[:, 0].float()), over="all", k=3)
