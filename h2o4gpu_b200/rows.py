@@ -12,9 +12,11 @@ and the gradients of each (``layer_norm_grad``, ``route_grad``, ``dispatch_grad`
 section 5 of include/h2o4gpu_kmeans.h: tensors are torch CUDA tensors (float32, float16 or bfloat16; ids int32), work is
 enqueued on the current stream of their device, nothing waits (``nearest`` does, as every call on a handle), nothing is
 kept between calls.  Outputs are new tensors of the caller's allocator.  Gradients are explicit functions: no call here
-records anything for autograd.  There is no CPU implementation.
+records anything for autograd, and one whose inputs require gradients while autograd records says so in a warning (call it
+under ``torch.no_grad()`` or on detached tensors).  There is no CPU implementation.
 """
 import ctypes
+import warnings
 from typing import NamedTuple
 
 import torch
@@ -175,6 +177,12 @@ def _out(out, like, index, rows, cols, exact=True):
     return out, _same_rows("out", out, like, index, (rows if exact or have < rows else have, cols))
 
 
+def _unrecorded(name):
+    """Warns that a call, some of whose inputs require gradients, cuts autograd's record."""
+    if torch.is_grad_enabled():
+        warnings.warn("%s records nothing for autograd: its result has no gradient, take %s_grad" % (name, name), stacklevel=3)
+
+
 def _over(over):
     if over not in _OVER:
         raise ValueError("over must be 'chosen' or 'all', not %r" % (over,))
@@ -210,6 +218,8 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, out=None):
         y, ystride = _out(out, x, index, rows, cols)
     mean = x.new_empty(rows, dtype=torch.float32)
     rstd = torch.empty_like(mean)
+    if x.requires_grad or (weight is not None and weight.requires_grad) or (bias is not None and bias.requires_grad):
+        _unrecorded("layer_norm")
     _call(_lib.kmeans_layer_norm, index, code, x.data_ptr(), stride, rows, cols, w, b, pcode, eps, y.data_ptr(), ystride,
           mean.data_ptr(), rstd.data_ptr())
     return LayerNorm(y, mean, rstd)
@@ -277,6 +287,8 @@ def route(scores, n, scale=-1.0, over="chosen"):
         raise ValueError("a row takes 1 to %d clusters, not %s" % (k, n))
     out = _routes(rows, n, scores)
     ids, weights, best, total = out
+    if scores.requires_grad:
+        _unrecorded("route")
     _call(_lib.kmeans_route, index, code, scores.data_ptr(), rs, cs, rows, k, n, scale, flag, ids.data_ptr(),
           weights.data_ptr(), best.data_ptr(), total.data_ptr())
     return out
@@ -394,6 +406,8 @@ def dispatch(x, plan, out=None):
     if have != rows:
         raise ValueError("x has %d rows, the plan %d" % (have, rows))
     y, ystride = _out(out, x, index, places, cols, exact=False)
+    if x.requires_grad:
+        _unrecorded("dispatch")
     _call(_lib.kmeans_dispatch, index, code, x.data_ptr(), stride, rows, cols, n, slot, source, places, y.data_ptr(), ystride)
     return y
 
@@ -414,6 +428,8 @@ def combine(rows, plan, weights=None, out=None):
         weights = _per_entry("weights", weights, index, torch.float32, (t, n))
     w = None if weights is None else weights.data_ptr()
     y, ystride = _out(out, rows, index, t, cols)
+    if rows.requires_grad or (weights is not None and weights.requires_grad):
+        _unrecorded("combine")
     _call(_lib.kmeans_combine, index, code, rows.data_ptr(), stride, places, cols, slot, w, t, n, y.data_ptr(), ystride)
     return y
 

@@ -3,6 +3,7 @@ test_rows.py."""
 import ctypes
 import os
 import subprocess
+import warnings
 
 import numpy as np
 import pytest
@@ -378,3 +379,28 @@ def test_route_grad_without_scores_refuses_what_is_not_on_a_gpu(built_lib):
         R.route_grad(ids.float(), None, R.Routes(ids, ids.float(), ids[:, 0].float(), ids[:, 0].float()), k=3)
     with pytest.raises(ValueError, match="needs the scores"):
         R.route_grad(ids.float(), None, R.Routes(ids, ids.float(), ids[:, 0].float(), ids[:, 0].float()), over="all", k=3)
+
+
+@gpu
+def test_a_call_that_cuts_autograd_warns(built_lib):
+    R = rows_module(built_lib)
+    x, s, w, wt = randn((6, 8), 260), randn((6, 5), 261), randn(8, 262), randn((6, 2), 263)
+    plan = R.sort_rows(torch.zeros((6, 2), dtype=torch.int32, device="cuda"), 3)
+    e = R.dispatch(x, plan)
+
+    def leaf(t):
+        return t.clone().requires_grad_()
+
+    calls = {"layer_norm": (lambda f: R.layer_norm(f(x))[0], lambda f: R.layer_norm(x, f(w))[0], lambda f: R.layer_norm(x, w, f(w))[0]),
+             "route": (lambda f: R.route(f(s), 2)[1],), "dispatch": (lambda f: R.dispatch(f(x), plan),),
+             "combine": (lambda f: R.combine(f(e), plan, wt), lambda f: R.combine(e, plan, f(wt)), lambda f: R.dispatch_grad(f(e), plan))}
+    for name, some in calls.items():
+        for call in some:
+            with pytest.warns(UserWarning, match=name + " records nothing for autograd.*" + name + "_grad"):
+                got = call(leaf)
+            with warnings.catch_warnings():
+                warnings.simplefilter("error")
+                want = call(lambda t: t)
+                with torch.no_grad():
+                    again = call(leaf)
+            assert torch.equal(got, want) and torch.equal(again, want) and not got.requires_grad
