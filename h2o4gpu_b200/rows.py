@@ -110,6 +110,8 @@ def _refuse(name, t, index=None, dtype=None, shape=None):
     """Raises what is wrong with a tensor that should be on device `index`, of `dtype` and `shape` (where they are given)."""
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
         raise ValueError("%s must be a CUDA tensor" % name)
+    if t.is_neg():
+        raise ValueError("%s is a view whose sign torch keeps apart: take its resolve_neg()" % name)
     if index is not None and t.get_device() != index:
         raise ValueError("%s is on %s, not on cuda:%d" % (name, t.device, index))
     if dtype is not None and t.dtype != dtype:
@@ -133,7 +135,7 @@ def _rows(name, t):
         stride, inner = t.stride()
     except (AttributeError, KeyError, ValueError):
         _refuse(name, t)
-    if index < 0 or (inner != 1 and cols > 1):
+    if index < 0 or (inner != 1 and (cols > 1 or t.is_neg())):
         _refuse(name, t)
     return rows, cols, stride if rows > 1 else cols, code, index
 
@@ -143,7 +145,7 @@ def _same_rows(name, t, like, index, shape):
     if not isinstance(t, torch.Tensor) or t.dtype is not like.dtype or t.get_device() != index or t.shape != shape:
         _refuse(name, t, index, like.dtype, shape)
     stride, inner = t.stride()
-    if inner != 1 and shape[1] > 1:
+    if inner != 1 and (shape[1] > 1 or t.is_neg()):
         _refuse(name, t, index, like.dtype, shape)
     return stride if shape[0] > 1 else shape[1]
 
@@ -260,7 +262,7 @@ def _scores(scores):
         rs, cs = scores.stride()
     except (AttributeError, KeyError, ValueError):
         _refuse("scores", scores)
-    if index < 0:
+    if index < 0 or scores.is_neg():
         _refuse("scores", scores)
     if k > _INT:
         raise ValueError("scores of %d clusters are too many" % k)
@@ -326,8 +328,8 @@ def route_grad(dweights, scores, routes, scale=-1.0, over="chosen", k=None, dtyp
         raise ValueError("routes of %d clusters a row, scores of %d" % (n, k))
     shape = (rows, n)
     dweights = _per_entry("dweights", dweights, index, f32, shape)
-    routes = (_per_entry("routes.ids", ids, index, torch.int32, shape), _per_entry("routes.weights", weights, index, f32, shape),
-              _per_entry("routes.best", best, index, f32, (rows,)), _per_entry("routes.total", total, index, f32, (rows,)))
+    ids, weights = _per_entry("routes.ids", ids, index, torch.int32, shape), _per_entry("routes.weights", weights, index, f32, shape)
+    best, total = _per_entry("routes.best", best, index, f32, (rows,)), _per_entry("routes.total", total, index, f32, (rows,))
     if rs < cs:
         out = dweights.new_empty((k, rows), dtype=dtype).t()
         drs, dcs = 1, rows
@@ -335,7 +337,7 @@ def route_grad(dweights, scores, routes, scale=-1.0, over="chosen", k=None, dtyp
         out = dweights.new_empty((rows, k), dtype=dtype)
         drs, dcs = k, 1
     _call(_lib.kmeans_route_grad, index, code, dweights.data_ptr(), None if scores is None else scores.data_ptr(), rs, cs, rows, k, n,
-          scale, flag, *[t.data_ptr() for t in routes], out.data_ptr(), drs, dcs)
+          scale, flag, ids.data_ptr(), weights.data_ptr(), best.data_ptr(), total.data_ptr(), out.data_ptr(), drs, dcs)
     return out
 
 

@@ -404,3 +404,19 @@ def test_a_call_that_cuts_autograd_warns(built_lib):
                 with torch.no_grad():
                     again = call(leaf)
             assert torch.equal(got, want) and torch.equal(again, want) and not got.requires_grad
+
+
+@gpu
+def test_views_whose_sign_is_kept_apart_are_refused(built_lib):
+    """The imaginary part of a conjugate: its memory holds the other sign."""
+    R = rows_module(built_lib)
+    z = torch.complex(randn((6, 5), 270), randn((6, 5), 271))
+    s = z.conj().imag
+    assert s.is_neg()
+    r = R.route(s.resolve_neg(), 2)
+    for call in (lambda: R.route(s, 2), lambda: R.route_grad(r.weights, s, r), lambda: R.layer_norm(s[:, :1]),
+                 lambda: R.layer_norm(z.imag[:, :1], out=s[:, :1])):
+        with pytest.raises(ValueError, match="resolve_neg"):
+            call()
+    check_route(R, s.resolve_neg(), 2, 1.0, "all")
+    check_route(R, z.imag, 2, 1.0, "all")                      # every second element
