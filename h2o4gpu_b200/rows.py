@@ -171,12 +171,31 @@ def _per_entry(name, t, index, dtype, shape):
     _refuse(name, t, index, dtype, shape)
 
 
-def _out(out, like, index, rows, cols, exact=True):
-    """The caller's output, or a new one of `like`'s type and device; and its row stride."""
+def _overlap(out, rows, t, t_rows):
+    """Whether the first `rows` rows of `out` share memory with the first `t_rows` of `t` (of the same type and as many columns); False too
+    for rows in two different strides, which are not looked at."""
+    cols, size = t.shape[1], t.element_size()
+    s, ts = (out.stride(0) if rows > 1 else 0), (t.stride(0) if t_rows > 1 else 0)
+    at = (t.data_ptr() - out.data_ptr()) // size
+    if not rows or not t_rows or at >= (rows - 1) * s + cols or at + (t_rows - 1) * ts + cols <= 0:
+        return False
+    if s and ts and s != ts:
+        return False
+    step = s or ts
+    return not step or not cols <= at % step <= step - cols      # columns side by side in rows of one stride
+
+
+def _out(out, like, index, rows, cols, exact=True, read=None, in_place=False):
+    """The caller's output, or a new one of `like`'s type and device; and its row stride.  `read`: rows of `like` that the call reads."""
     if out is None:
         return like.new_empty((rows, cols)), cols
     have = out.shape[0] if isinstance(out, torch.Tensor) and out.dim() == 2 else rows
-    return out, _same_rows("out", out, like, index, (rows if exact or have < rows else have, cols))
+    stride = _same_rows("out", out, like, index, (rows if exact or have < rows else have, cols))
+    read = like.shape[0] if read is None else read
+    same = in_place and out.data_ptr() == like.data_ptr() and (rows < 2 or stride == like.stride(0))
+    if not same and _overlap(out, rows, like, read):
+        raise ValueError("out shares memory with the rows that are read")
+    return out, stride
 
 
 def _unrecorded(name):
@@ -217,7 +236,7 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, out=None):
     if out is None and stride == cols:
         y, ystride = torch.empty_like(x), cols
     else:
-        y, ystride = _out(out, x, index, rows, cols)
+        y, ystride = _out(out, x, index, rows, cols, in_place=True)
     mean = x.new_empty(rows, dtype=torch.float32)
     rstd = torch.empty_like(mean)
     if x.requires_grad or (weight is not None and weight.requires_grad) or (bias is not None and bias.requires_grad):
@@ -429,7 +448,7 @@ def combine(rows, plan, weights=None, out=None):
     if weights is not None:
         weights = _per_entry("weights", weights, index, torch.float32, (t, n))
     w = None if weights is None else weights.data_ptr()
-    y, ystride = _out(out, rows, index, t, cols)
+    y, ystride = _out(out, rows, index, t, cols, read=places)
     if rows.requires_grad or (weights is not None and weights.requires_grad):
         _unrecorded("combine")
     _call(_lib.kmeans_combine, index, code, rows.data_ptr(), stride, places, cols, slot, w, t, n, y.data_ptr(), ystride)

@@ -420,3 +420,56 @@ def test_views_whose_sign_is_kept_apart_are_refused(built_lib):
             call()
     check_route(R, s.resolve_neg(), 2, 1.0, "all")
     check_route(R, z.imag, 2, 1.0, "all")                      # every second element
+
+
+@gpu
+def test_outputs_on_the_memory_of_their_inputs(built_lib):
+    """Rows are read while others are written: an output that shares memory with them is refused, but for the norm in place; parts of one
+    buffer beside each other are not."""
+    R = rows_module(built_lib)
+    buf = randn((64, 40), 280)
+    plan = R.sort_rows(torch.arange(16, device="cuda", dtype=torch.int32).view(8, 2) % 3, 3)       # 16 places for 8 rows
+    x, e = buf[:8, :16], buf[:16, :16]
+    for call in (lambda: R.layer_norm(x, out=buf[1:9, :16]), lambda: R.layer_norm(x, out=buf[:8, 4:20]), lambda: R.layer_norm(buf[:1, :16], out=buf[:1, 15:31]),
+                 lambda: R.layer_norm(buf.view(-1)[:128].view(8, 16), out=buf.view(-1)[16:144].view(8, 16)),
+                 lambda: R.dispatch(x, plan, out=buf[:16, :16]), lambda: R.dispatch(x, plan, out=buf[7:23, :16]),
+                 lambda: R.dispatch(x, plan, out=buf[:, :16]), lambda: R.combine(e, plan, out=x), lambda: R.combine(e, plan, out=buf[15:23, :16]),
+                 lambda: R.dispatch_grad(e, plan, out=x), lambda: R.dispatch(buf[3:4, 8:24].expand(8, 16), plan, out=buf[:16, :16])):
+        with pytest.raises(ValueError, match="shares memory"):
+            call()
+    want = R.layer_norm(x).y
+    keep = buf.clone()
+    for out in (buf[8:16, :16], buf[:8, 16:32], buf[1:9, 20:36], buf[:8, 24:40], buf[20:28, 3:19], x):
+        assert torch.equal(R.layer_norm(x, out=out).y, want)
+        buf.copy_(keep)
+    want = R.dispatch(x, plan)
+    for out in (buf[8:24, :16], buf[:16, 16:32], buf[8:, :16], buf[:, 24:]):
+        assert torch.equal(R.dispatch(x, plan, out=out)[:16], want)
+        buf.copy_(keep)
+    for rows, out in ((e, buf[16:24, :16]), (buf[:, :16], buf[16:24, :16]), (e, buf[:8, 16:32]), (buf[::2, :16], buf[1:17:2, :16])):
+        assert torch.equal(R.combine(rows, plan, out=out), R.combine(rows.clone(), plan))
+        buf.copy_(keep)
+
+
+def test_overlap_rule_against_sets_of_addresses(built_lib):
+    from h2o4gpu_b200.rows import _overlap
+    rng = np.random.default_rng(1)
+    buf = torch.zeros(400)
+    seen = [0, 0]
+    for _ in range(4000):
+        cols = int(rng.integers(1, 9))
+
+        def view(zero):
+            rows, step = int(rng.integers(1, 6)), int(rng.choice([0, cols, cols + 1, cols + 5, 2 * cols, 20]))
+            return buf.as_strided((rows if step or zero else 1, cols), (max(step, cols) if step else 0, 1), int(rng.integers(0, 120)))
+
+        a, b = view(False), view(True)
+        sa, sb = a.stride(0) * (a.shape[0] > 1), b.stride(0) * (b.shape[0] > 1)
+        places = [{t.storage_offset() + i * t.stride(0) + j for i in range(t.shape[0]) for j in range(cols)} for t in (a, b)]
+        shared = bool(places[0] & places[1])
+        if not (sa and sb and sa != sb):
+            assert _overlap(a, a.shape[0], b, b.shape[0]) == shared
+            seen[shared] += 1
+        else:
+            assert not _overlap(a, a.shape[0], b, b.shape[0])
+    assert min(seen) > 300
