@@ -106,8 +106,8 @@ struct ResidentCtas {
   }
 };
 
-// A kernel that is put in place while the one before it on the stream still runs; it has to wait for that one (wait_for_previous) before it
-// touches memory.
+// A kernel that is put in place while the one before it on the stream still runs.  Before it waits for that one (wait_for_previous) it may
+// read only what was there when that one began - an input of both - and write nothing but its own shared memory.
 template <typename... P, typename... A>
 int launch_early(void (*fn)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, A... args) {
   cudaLaunchAttribute attr;

@@ -47,8 +47,10 @@ __device__ __forceinline__ float route_value(T s, float sign) {
   return fminf(fmaxf(sign * to_f(s), -INFINITY), 3.402823466e38f);      // (the maximum of NaN and a number is the number)
 }
 
-// exp(x), x <= 0, for sums of many terms: 2^(x log2 e) with the product rounded once more than in expf, which puts |x| 2^-24 of a term
-// on top - at most 0.4 2^-24 of the largest one, as x e^-x is - for a third of the instructions.
+// exp(x), x = a d <= 0, for sums of many terms, for a third of expf's instructions: 2^(a2 d) with a2 = a log2 e.  log2 e as a float32 is off by 0.22
+// 2^-24 of itself, a2 and a2 d are rounded: the exponent is off by 2.22 |x| 2^-24 at most (1.22 where a is 1), which puts 0.82 2^-24 of the
+// largest term on a term, as |x| e^x is below 0.37, besides ex2's own error.  (a2 stops at the largest
+// float32, for scales above 2.3e38.)
 __device__ __forceinline__ float exp2_fast(float x) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
