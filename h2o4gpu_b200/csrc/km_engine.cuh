@@ -797,6 +797,7 @@ int Engine<T>::upload_host_typed(const void* Xv, int src_dtype, size_t rows, siz
   if (order != 'r' && order != 'c') KM_FAIL(KM_EINVAL, "kmeans_upload_host: order must be 'r' or 'c'");
   if (world_size != (int)shards.size())
     KM_FAIL(KM_ESTATE, "kmeans_upload_host: one process must own all ranks; use kmeans_attach_device");
+  if (rows < shards.size()) KM_FAIL(KM_EINVAL, "kmeans_upload_host: fewer rows than devices");
   KM_TRY(upload_wait());
   const bool native = src_dtype == (sizeof(T) == 8 ? KM_DTYPE_F64 : KM_DTYPE_F32);
   const unsigned char* X = static_cast<const unsigned char*>(Xv);
@@ -837,7 +838,6 @@ int Engine<T>::upload_host_typed(const void* Xv, int src_dtype, size_t rows, siz
   for (size_t i = 0; i < g; ++i) {
     Shard<T>& s = shards[i];
     const size_t r = per + (i < extra ? 1 : 0);
-    if (r == 0) { upload_wait(); KM_FAIL(KM_EINVAL, "kmeans_upload_host: fewer rows than devices"); }
     DevGuard gd(s.dev);
     s.X = nullptr;      // until the new matrix is attached the shard has none
     s.rows = 0;

@@ -81,9 +81,13 @@ class ResidentKMeans(object):
             order = 'c' if (X.flags.f_contiguous and not X.flags.c_contiguous) else 'r'
         X = np.ascontiguousarray(X) if order == 'r' else np.asfortranarray(X)
         rows, cols = X.shape
-        self._rows = [0] * self.n_local           # what a failed upload leaves
-        _lk.check(self._lib.kmeans_upload_host_typed(self._h, X.ctypes.data_as(ctypes.c_void_p),
-                                                     DTYPE_CODES[X.dtype], rows, cols, order.encode()))
+        try:
+            _lk.check(self._lib.kmeans_upload_host_typed(self._h, X.ctypes.data_as(ctypes.c_void_p),
+                                                         DTYPE_CODES[X.dtype], rows, cols, order.encode()))
+        except _lk.KMeansLibError as e:
+            if e.code not in (_lk.EINVAL, _lk.ESTATE):      # refused before anything was touched; else there is no matrix any more
+                self._rows = [0] * self.n_local
+            raise
         per, extra = divmod(rows, self.n_local)   # the library's balanced contiguous split
         self._rows = [per + (1 if i < extra else 0) for i in range(self.n_local)]
         self.cols = cols

@@ -24,7 +24,9 @@ _vp = _c.c_void_p
 _ll = _c.c_longlong
 
 
+EINVAL = -1          # KM_EINVAL
 ENONFINITE = -6      # KM_ENONFINITE
+ESTATE = -8          # KM_ESTATE
 
 
 class KMeansLibError(RuntimeError):

@@ -106,8 +106,8 @@ def test_combine_grad_addresses_only_rows_that_are_there(tmp_path):
 def test_combine_grad_of_rows_that_do_not_fill_a_cta(built_lib, dtype):
     """Rows of dy far apart, one to seven of them: results as from rows side by side."""
     R = rows_module(built_lib)
-    n, k, d = 4, 6, 64
-    for rows in range(1, 8):
+    n, k = 4, 6
+    for rows, d in [(r, c) for r in range(1, 8) for c in (64, 256, 400, 1024)]:      # one, two and four warps a row
         plan = R.sort_rows(make_ids(rows, n, k, 206), k, 2)
         e, w, dy = randn((plan.source.shape[0], d), 207, dtype), randn((rows, n), 208), randn((rows, d), 209, dtype)
         apart = torch.zeros((rows, 50, d), dtype=dtype, device="cuda")
@@ -359,6 +359,9 @@ def test_nearest_after_a_failed_attach_or_upload(built_lib):
             lib.kmeans_selftest_alloc_limit(-1)
 
     fails(lambda: h.attach_device(0, many.data_ptr(), 200_000, 16))
+    assert all(torch.equal(a, b) for a, b in zip(R.nearest(h, 3), want)) and np.array_equal(h.labels(), labels)
+    with pytest.raises(RuntimeError):
+        h.upload(np.empty((0, 16), np.float32))      # refused: nothing has changed
     assert all(torch.equal(a, b) for a, b in zip(R.nearest(h, 3), want)) and np.array_equal(h.labels(), labels)
     fails(lambda: h.upload(many.cpu().numpy()))
     for call in (lambda: R.nearest(h, 3), h.transform, h.labels, lambda: h.fit(few[:7].cpu().numpy(), 2), h.assign):
